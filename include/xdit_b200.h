@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define XDIT_ABI_VERSION 3
+#define XDIT_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define XDIT_API __attribute__((visibility("default")))
@@ -338,6 +338,108 @@ struct xdit_prologue_params {
   int64_t dst_stride_h[3], dst_stride_b[3];
 };
 XDIT_API int xdit_qk_norm_rope_pack(const struct xdit_prologue_params* p, void* stream);
+
+/* Rotary positions with several axes.  A head's first 2*pairs elements are rotated, the rest pass: pair i
+ * is (2i, 2i+1), or (i, i + pairs) with `halves`, and turns by position(token, axis[i]) * frequencies[i]
+ * radians: (a, b) -> (a cos - b sin, a sin + b cos).  Positions come from memory, or from a grid that the
+ * token index start + row walks with its last axis running fastest (tokens behind the grid are not rotated).
+ * frequencies and axis are HOST arrays of `pairs` entries, read during the call.
+ * Replaces: the inline apply_rotary_emb and the position tables of the processors
+ * (transformer_wan.py:106-122, the frequencies' chunk at :311-319). */
+#define XDIT_ROTARY_MAX_PAIRS 256
+#define XDIT_ROTARY_MAX_AXES 4
+enum xdit_position_kind { XDIT_POS_GRID = 0, XDIT_POS_I32 = 1, XDIT_POS_I64 = 2, XDIT_POS_F32 = 3 };
+struct xdit_rotary_positions {
+  int32_t kind, axes, pairs;
+  const double* frequencies; /* host */
+  const uint8_t* axis;       /* host */
+  const void* positions;     /* device, NULL for a grid */
+  int64_t stride_b, stride_row, stride_axis; /* elements; stride_b 0: the same for every sample */
+  int64_t grid[XDIT_ROTARY_MAX_AXES], start;
+};
+/* q [B, H, s, D] and k [B, Hk, s, D] (Hk = 0: no k) by strides, into out_q and out_k, which may be q and k
+ * themselves but not overlap them in another way.  Any dtype, stride and alignment. */
+struct xdit_rotary_params {
+  int32_t dtype, B, H, Hk, s, D;
+  int32_t halves;
+  struct xdit_rotary_positions pos;
+  const void *q, *k;
+  void *out_q, *out_k;
+  int64_t stride_b[2], stride_h[2], stride_row[2];             /* of q and k */
+  int64_t out_stride_b[2], out_stride_h[2], out_stride_row[2]; /* of out_q and out_k */
+};
+XDIT_API int xdit_rotary_axes(const struct xdit_rotary_params* p, void* stream);
+/* The same angles as the cos and sin tables that xdit_qk_norm_rope_pack takes: fp32 [s, D] contiguous, each
+ * value at both elements of its interleaved pair, 1 and 0 behind the rotated part. */
+XDIT_API int xdit_rotary_tables(const struct xdit_rotary_positions* pos, float* cos, float* sin, int32_t s,
+                                int32_t D, void* stream);
+
+/* The steps of a DiT block between two sub-layers, in one pass over each token's row of C values:
+ *   out_residual = residual_scale * residual + gate * post_norm(branch)     (without a branch: residual itself)
+ *   out          = norm(...) * (1 + scale) + shift
+ * with norms XDIT_NORM_NONE, _LAYER (mean and variance) or _RMS, each with an optional weight and bias.  norm
+ * takes the unrounded sum.  Rows of modulation (xdit_row_vec, NULL ptr: absent) hold C contiguous values in
+ * `dtype` or fp32; their strides are 0 where samples or tokens share a row.  post_weight, post_bias, weight
+ * and bias are shared by all rows.  out_residual may be residual or branch itself.
+ * With out_q the second result is written as e4m3 rows instead of `out`: [B*s, C] bytes and one scale
+ * for each block of 128, out_scale[block * out_scale_ld + row]; needs C % 16 == 0 and 16-byte aligned rows.
+ * Replaces: norm1/norm2 + modulation + gated residual around the attention and the MLP of the blocks that
+ * transformer_wan.py:321-336 and transformer_flux.py:300-330 run. */
+#define XDIT_NORM_MAX_C 16384
+#define XDIT_FP8_BLOCK 128
+enum xdit_norm_kind { XDIT_NORM_NONE = 0, XDIT_NORM_LAYER = 1, XDIT_NORM_RMS = 2 };
+struct xdit_row_vec {
+  const void* ptr;
+  int64_t stride_b, stride_row;
+  int32_t dtype;
+};
+struct xdit_norm_params {
+  int32_t dtype, B, s, C;
+  int32_t post_norm, norm;
+  float residual_scale, eps;
+  const void *residual, *branch;
+  int64_t residual_stride_b, residual_stride_row, branch_stride_b, branch_stride_row;
+  void *out_residual, *out;
+  int64_t out_residual_stride_b, out_residual_stride_row, out_stride_b, out_stride_row;
+  void* out_q;
+  float* out_scale;
+  int64_t out_scale_ld;
+  struct xdit_row_vec post_weight, post_bias, gate, weight, bias, scale, shift;
+};
+XDIT_API int xdit_gated_residual_norm(const struct xdit_norm_params* p, void* stream);
+
+/* e4m3 with one fp32 scale for each block of 128.  The scale is the smallest power of two that brings a
+ * block within 448 (1 for a block of zeros, NaN for a block with an infinity or a NaN), so a value
+ * is rounded once.  Rows: x [B, s, K] -> q [B*s, K], scale[block * scale_ld + row].  Weight: w [N, K] ->
+ * q [N, K], scale [N/128 rounded up][K/128 rounded up], blocks of 128 x 128.  K % 16 == 0, 16-byte aligned rows. */
+XDIT_API int xdit_quantize_rows(const void* x, int64_t stride_b, int64_t stride_row, int32_t dtype, int32_t B,
+                                int32_t s, int32_t K, void* q, float* scale, int64_t scale_ld, void* stream);
+XDIT_API int xdit_quantize_weight(const void* w, int64_t stride_row, int32_t dtype, int32_t N, int32_t K, void* q,
+                                  float* scale, void* stream);
+
+/* out[m, n] = act(sum_c x_scale[m, c] w_scale[n/128, c] sum_{k in block c} x[m, k] w[n, k] + bias[n]) with x
+ * [M, K] and w [N, K] in e4m3 and scales of any value.  out: bf16, fp16 or fp32, rounded once; or, with
+ * out_q, e4m3 rows [M, N] with out_scale[block * out_scale_ld + row] (N % 16 == 0).  K % 16 == 0; rows of x and
+ * w start on 16-byte boundaries.  status, status_host and wait_limit_ns as in xdit_attn_params.
+ * Replaces: the fp8 linear layers of xfuser/model_executor/layers/fp8_linear.py. */
+enum xdit_activation { XDIT_ACT_NONE = 0, XDIT_ACT_GELU_TANH = 1 };
+struct xdit_fp8_linear_params {
+  int32_t M, N, K;
+  int32_t activation, out_dtype, bias_dtype;
+  const void *x, *w;
+  int64_t x_stride_row, w_stride_row;
+  const float *x_scale, *w_scale;
+  int64_t x_scale_stride_row, x_scale_stride_block, w_scale_stride_row, w_scale_stride_block;
+  const void* bias;
+  void* out;
+  int64_t out_stride_row;
+  void* out_q;
+  float* out_scale;
+  int64_t out_scale_ld;
+  int32_t *status, *status_host;
+  uint32_t wait_limit_ns;
+};
+XDIT_API int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,12 @@ XDIT_BF16, XDIT_F16, XDIT_F32 = 0, 1, 2
 XDIT_MAX_PACK_JOBS = 4
 XDIT_MAX_OUT_SEGMENTS = 16
 XDIT_PEER_HANDLE_BYTES = 64
+XDIT_POS_GRID, XDIT_POS_I32, XDIT_POS_I64, XDIT_POS_F32 = 0, 1, 2, 3
+XDIT_ROTARY_MAX_PAIRS, XDIT_ROTARY_MAX_AXES = 256, 4
+XDIT_NORM_NONE, XDIT_NORM_LAYER, XDIT_NORM_RMS = 0, 1, 2
+XDIT_NORM_MAX_C = 16384
+XDIT_FP8_BLOCK = 128
+XDIT_ACT_NONE, XDIT_ACT_GELU_TANH = 0, 1
 XDIT_STATIC_ACC_FLOATS = 8 * 1024 * 1024
 
 EXPORTS = [
@@ -42,10 +48,16 @@ EXPORTS = [
     "xdit_seq_gather_unpad",
     "xdit_merge_out_lse",
     "xdit_qk_norm_rope_pack",
+    "xdit_rotary_axes",
+    "xdit_rotary_tables",
+    "xdit_gated_residual_norm",
+    "xdit_quantize_rows",
+    "xdit_quantize_weight",
+    "xdit_fp8_linear",
 ]
 
 
-ABI_VERSION = 3  # XDIT_ABI_VERSION of include/xdit_b200.h: the structures below mirror that header
+ABI_VERSION = 4  # XDIT_ABI_VERSION of include/xdit_b200.h: the structures below mirror that header
 
 
 class Caps(C.Structure):
@@ -116,6 +128,62 @@ class PrologueParams(C.Structure):
         ("dst_q", C.c_void_p), ("dst_k", C.c_void_p), ("dst_v", C.c_void_p),
         ("dst_q_peer_stride", C.c_int64), ("dst_k_peer_stride", C.c_int64), ("dst_v_peer_stride", C.c_int64),
         ("dst_stride_h", C.c_int64 * 3), ("dst_stride_b", C.c_int64 * 3),
+    ]
+
+
+class RotaryPositions(C.Structure):
+    _fields_ = [
+        ("kind", C.c_int32), ("axes", C.c_int32), ("pairs", C.c_int32),
+        ("frequencies", C.POINTER(C.c_double)), ("axis", C.POINTER(C.c_uint8)),
+        ("positions", C.c_void_p),
+        ("stride_b", C.c_int64), ("stride_row", C.c_int64), ("stride_axis", C.c_int64),
+        ("grid", C.c_int64 * XDIT_ROTARY_MAX_AXES), ("start", C.c_int64),
+    ]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("Hk", C.c_int32), ("s", C.c_int32),
+        ("D", C.c_int32), ("halves", C.c_int32),
+        ("pos", RotaryPositions),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("out_q", C.c_void_p), ("out_k", C.c_void_p),
+        ("stride_b", C.c_int64 * 2), ("stride_h", C.c_int64 * 2), ("stride_row", C.c_int64 * 2),
+        ("out_stride_b", C.c_int64 * 2), ("out_stride_h", C.c_int64 * 2), ("out_stride_row", C.c_int64 * 2),
+    ]
+
+
+class RowVec(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_b", C.c_int64), ("stride_row", C.c_int64), ("dtype", C.c_int32)]
+
+
+class NormParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("s", C.c_int32), ("C", C.c_int32),
+        ("post_norm", C.c_int32), ("norm", C.c_int32), ("residual_scale", C.c_float), ("eps", C.c_float),
+        ("residual", C.c_void_p), ("branch", C.c_void_p),
+        ("residual_stride_b", C.c_int64), ("residual_stride_row", C.c_int64),
+        ("branch_stride_b", C.c_int64), ("branch_stride_row", C.c_int64),
+        ("out_residual", C.c_void_p), ("out", C.c_void_p),
+        ("out_residual_stride_b", C.c_int64), ("out_residual_stride_row", C.c_int64),
+        ("out_stride_b", C.c_int64), ("out_stride_row", C.c_int64),
+        ("out_q", C.c_void_p), ("out_scale", C.c_void_p), ("out_scale_ld", C.c_int64),
+        ("post_weight", RowVec), ("post_bias", RowVec), ("gate", RowVec), ("weight", RowVec), ("bias", RowVec),
+        ("scale", RowVec), ("shift", RowVec),
+    ]
+
+
+class Fp8LinearParams(C.Structure):
+    _fields_ = [
+        ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+        ("activation", C.c_int32), ("out_dtype", C.c_int32), ("bias_dtype", C.c_int32),
+        ("x", C.c_void_p), ("w", C.c_void_p), ("x_stride_row", C.c_int64), ("w_stride_row", C.c_int64),
+        ("x_scale", C.c_void_p), ("w_scale", C.c_void_p),
+        ("x_scale_stride_row", C.c_int64), ("x_scale_stride_block", C.c_int64),
+        ("w_scale_stride_row", C.c_int64), ("w_scale_stride_block", C.c_int64),
+        ("bias", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride_row", C.c_int64),
+        ("out_q", C.c_void_p), ("out_scale", C.c_void_p), ("out_scale_ld", C.c_int64),
+        ("status", C.c_void_p), ("status_host", C.c_void_p), ("wait_limit_ns", C.c_uint32),
     ]
 
 
@@ -191,6 +259,21 @@ def load() -> C.CDLL:
     lib.xdit_merge_out_lse.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
     lib.xdit_merge_out_lse.restype = C.c_int
+    lib.xdit_rotary_axes.argtypes = [C.POINTER(RotaryParams), C.c_void_p]
+    lib.xdit_rotary_axes.restype = C.c_int
+    lib.xdit_rotary_tables.argtypes = [C.POINTER(RotaryPositions), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                       C.c_void_p]
+    lib.xdit_rotary_tables.restype = C.c_int
+    lib.xdit_gated_residual_norm.argtypes = [C.POINTER(NormParams), C.c_void_p]
+    lib.xdit_gated_residual_norm.restype = C.c_int
+    lib.xdit_quantize_rows.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                       C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+    lib.xdit_quantize_rows.restype = C.c_int
+    lib.xdit_quantize_weight.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
+                                         C.c_void_p, C.c_void_p]
+    lib.xdit_quantize_weight.restype = C.c_int
+    lib.xdit_fp8_linear.argtypes = [C.POINTER(Fp8LinearParams), C.c_void_p]
+    lib.xdit_fp8_linear.restype = C.c_int
     _lib = lib
     return lib
 

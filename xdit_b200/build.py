@@ -16,7 +16,9 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 LIB = os.path.join(PKG, "libxdit_b200.so")
 OBJ = os.path.join(PKG, "csrc", "_obj")
-SOURCES = ["capi.cu", "rowcopy.cu", "merge.cu", "attn_generic.cu", "attn_sm100.cu", "attn_static_acc.cu", "prologue.cu", "peer_barrier.cu"]
+SOURCES = ["capi.cu", "rowcopy.cu", "merge.cu", "attn_generic.cu", "attn_sm100.cu", "attn_static_acc.cu", "prologue.cu", "peer_barrier.cu",
+           "rotary.cu", "modnorm.cu", "fp8_gemm.cu"]
+HEADERS = ["common.cuh", "sm100_ptx.cuh", "fp8_quant.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -32,7 +34,7 @@ def _nvcc() -> str:
 
 def _deps():
     files = [os.path.join(CSRC, s) for s in SOURCES]
-    files += [os.path.join(CSRC, "common.cuh"), os.path.join(INCLUDE, "xdit_b200.h")]
+    files += [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "xdit_b200.h")]
     return files
 
 

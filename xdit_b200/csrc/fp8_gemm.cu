@@ -1,0 +1,395 @@
+// y = act(x W^T + bias) with x [M, K] and W [N, K] in e4m3 and one fp32 scale for each block of 128 along K
+// (of every row of x; of every 128 rows of W):
+//   y[m, n] = sum_c xs[m, c] ws[n / 128, c] sum_{k in block c} x[m, k] w[n, k]
+// The inner sums run on the tensor cores (tcgen05.mma kind::f8f6f4, fp32 accumulators in TMEM); the scales
+// differ from block to block, so every inner sum is taken out of TMEM, scaled and added in registers.
+//
+// One CTA per SM walks output tiles of 128 rows x 256 columns.  A step is one block of 128 along K, which
+// is also one 128-byte swizzle row of the operands in shared memory:
+//   warp 9     loads the step's operands by TMA (16 KB of x, 32 KB of W) into a ring
+//   warp 8     issues the step's four MMAs (128 x 256 x 32) into one of two TMEM buffers of 256 columns
+//   warps 0-7  two warpgroups, 128 columns each: thread = row, 128 fp32 sums in registers; they add the
+//              scaled buffer of one step while the tensor core fills the other
+// A warpgroup's columns share ws, so the scale of a step is one product per thread.  After the last step the
+// sums get bias and activation and are written, rounded once; or they become e4m3 rows again: a
+// thread holds a whole block of 128 of its row, so that block's scale needs no exchange.
+//
+// Every wait on an mbarrier is bounded in time; when one gives up the CTA raises a flag in shared memory, all
+// roles leave their loops, outstanding copies and MMAs are drained with bounded waits, TMEM is freed and
+// *status is set.
+#include <cstring>
+#include <mutex>
+
+#include "fp8_quant.cuh"
+#include "sm100_ptx.cuh"
+
+namespace xdit {
+namespace {
+
+constexpr int kThreads = 384;  // 8 summing warps, MMA warp, TMA warp, 2 idle warps (full register-trading warpgroup)
+constexpr int kBM = 128, kBN = 256, kBK = XDIT_FP8_BLOCK;
+constexpr int kStages = 4;
+constexpr int kABytes = kBM * kBK, kBBytes = kBN * kBK, kStageBytes = kABytes + kBBytes;
+constexpr int kBarOff = kStages * kStageBytes;
+constexpr int kNumBars = 2 * kStages + 4 + 1;
+constexpr int kMiscOff = kBarOff + kNumBars * 8;
+constexpr int kSmem = kMiscOff + 16 + 1024;  // with slack to align the base to 1024 bytes
+constexpr int kBand = 16;                    // row tiles of a band: tiles of a band are walked column by column
+
+struct alignas(64) GemmArgs {
+  CUtensorMap tm_x, tm_w;
+  int32_t M, N, kb;        // kb: blocks along K
+  int32_t mt, nt;          // tiles
+  const float* xs;
+  int64_t xs_srow, xs_skb;
+  const float* ws;
+  int64_t ws_snb, ws_skb;
+  const void* bias;
+  int32_t bias_dtype, act, out_dtype;
+  void* out;
+  int64_t out_srow;
+  uint8_t* out_q;
+  float* out_scale;
+  int64_t out_scale_ld;
+  int32_t wide;            // 16-byte stores are possible
+  int32_t* status;
+  int32_t* status_host;
+  uint32_t wait_limit_ns;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  if (dtype == XDIT_F32) return __ldg(reinterpret_cast<const float*>(p) + i);
+  if (dtype == XDIT_BF16) return __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p) + i));
+  return __half2float(__ldg(reinterpret_cast<const __half*>(p) + i));
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x) {
+  if (dtype == XDIT_F32) reinterpret_cast<float*>(p)[i] = x;
+  else if (dtype == XDIT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+// x/2 (1 + tanh u) = x / (1 + exp(-2u)) with u = sqrt(2/pi) (x + 0.044715 x^3)
+__device__ __forceinline__ float gelu_tanh(float x) {
+  const float u = 0.7978845608028654f * fmaf(0.044715f * x * x, x, x);
+  return __fdividef(x, 1.f + __expf(-2.f * u));
+}
+__device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& m, int& n) {
+  const int band = t / (kBand * a.nt), rem = t - band * kBand * a.nt;
+  const int rows = min(kBand, a.mt - band * kBand);
+  n = rem / rows;
+  m = band * kBand + rem - n * rows;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_constant__ GemmArgs a) {
+  extern __shared__ unsigned char smem_dyn[];
+  const uint32_t raw = smem_u32(smem_dyn), base = (raw + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_dyn + (base - raw);
+  const uint32_t bar0 = base + kBarOff;
+  auto bar_full = [&](int s) { return bar0 + 8u * s; };
+  auto bar_empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto bar_tfull = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
+  auto bar_tempty = [&](int s) { return bar0 + 8u * (2 * kStages + 2 + s); };
+  const uint32_t bar_drain = bar0 + 8u * (2 * kStages + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + kMiscOff + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = a.mt * a.nt;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(bar_tfull(s), 1); mbar_init(bar_tempty(s), 256); }
+    mbar_init(bar_drain, 1);
+    *abort_flag = status_is_set(a.status) ? -1 : 0;  // -1: skip all work (an earlier failure is pending)
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool skip = *abort_flag != 0;  // same value for every thread: written before the barrier above
+
+  if (skip) {
+    // nothing to do: fall through to the teardown, which frees TMEM
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");  // 2 x 232 + 40 <= 512 per scheduler
+    if (warp == 9) {
+      // ======================= TMA producer =======================
+      if (lane == 0) {
+        int issued = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+          int m, n;
+          tile_at(a, t, m, n);
+          for (int c = 0; c < a.kb; ++c) {
+            const int st = issued % kStages, turn = issued / kStages;
+            if (turn > 0) ok = mbar_wait(bar_empty(st), (turn - 1) & 1, abort_flag, a.wait_limit_ns, 100 + st);
+            if (!ok) break;
+            mbar_arrive_expect_tx(bar_full(st), kStageBytes);
+            tma_load_2d(base + st * kStageBytes, &a.tm_x, bar_full(st), c * kBK, m * kBM);
+            tma_load_2d(base + st * kStageBytes + kABytes, &a.tm_w, bar_full(st), c * kBK, n * kBN);
+            ++issued;
+          }
+        }
+        if (!ok) {
+          // drain: every armed stage must have received its bytes before the CTA may leave
+          for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+            for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_full(i % kStages), (i / kStages) & 1); ++it) __nanosleep(64);
+        }
+      }
+    } else if (warp == 8) {
+      // ======================= MMA issuer (the warp runs converged, one elected lane issues) =======================
+      const bool leader = elect_one();
+      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t idesc = (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> fp32
+      bool ok = true;
+      int step = 0;
+      auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.wait_limit_ns, code));
+      };
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (int c = 0; c < a.kb; ++c, ++step) {
+          const int st = step % kStages, buf = step & 1;
+          if (step >= 2) ok = wait_all(bar_tempty(buf), ((step >> 1) - 1) & 1, 200 + buf);
+          if (ok) ok = wait_all(bar_full(st), (step / kStages) & 1, 210 + st);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t da = desc_kmajor(base + st * kStageBytes), db = desc_kmajor(base + st * kStageBytes + kABytes);
+#pragma unroll
+            for (int k = 0; k < kBK / 32; ++k) mma_f8(tmem_u + buf * kBN, da + 2 * k, db + 2 * k, idesc, k > 0);
+            tc_commit(bar_empty(st));
+            tc_commit(bar_tfull(buf));
+          }
+        }
+      }
+      if (!ok) {
+        // drain the tensor pipe before TMEM is released
+        if (leader) tc_commit(bar_drain);
+        if (lane == 0)
+          for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_drain, 0); ++it) __nanosleep(64);
+        __syncwarp();
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    // ======================= scaled sums + epilogue =======================
+    const int half = warp >> 2;  // columns [128 half, 128 half + 128) of the tile
+    const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
+    const int row_in = (warp & 3) * 32 + lane;
+    bool ok = true;
+    int step = 0;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int m, n;
+      tile_at(a, t, m, n);
+      const int64_t row = (int64_t)m * kBM + row_in;
+      const int col0 = n * kBN + half * 128;
+      const bool live = row < a.M && col0 < a.N;
+      const float* xs = a.xs + (live ? row : 0) * a.xs_srow;
+      const float* ws = a.ws + (live ? col0 / kBK : 0) * a.ws_snb;
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      float sx = __ldg(xs), sw = __ldg(ws);
+      for (int c = 0; c < a.kb; ++c, ++step) {
+        const int buf = step & 1;
+        const float s = live ? sx * sw : 0.f;
+        if (c + 1 < a.kb) { sx = __ldg(xs + (c + 1) * a.xs_skb); sw = __ldg(ws + (c + 1) * a.ws_skb); }
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull(buf), (step >> 1) & 1, abort_flag, a.wait_limit_ns, 300 + buf));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t p[32];
+          XDIT_TMEM_LD32(p, 0, taddr + buf * kBN + 32 * q);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[32 * q + i] = fmaf(s, __uint_as_float(p[i]), acc[32 * q + i]);
+        }
+        tc_fence_before();
+        mbar_arrive(bar_tempty(buf));
+      }
+      if (!ok || !live) continue;
+      if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (col0 + i < a.N) acc[i] += load_any(a.bias, a.bias_dtype, col0 + i);
+      }
+      if (a.act == XDIT_ACT_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] = gelu_tanh(acc[i]);
+      }
+      if (a.out_q) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (col0 + i < a.N) top = amax_nan(top, acc[i]);
+        float inv;
+        a.out_scale[(col0 / kBlock) * a.out_scale_ld + row] = block_scale(top, inv);
+        uint8_t* o = a.out_q + row * a.N + col0;
+#pragma unroll
+        for (int i = 0; i < 128; i += 16) {
+          if (col0 + i >= a.N) break;  // N is a multiple of 16 here
+          uint4 w;
+          w.x = pack_e4m3(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+          w.y = pack_e4m3(acc[i + 4] * inv, acc[i + 5] * inv, acc[i + 6] * inv, acc[i + 7] * inv);
+          w.z = pack_e4m3(acc[i + 8] * inv, acc[i + 9] * inv, acc[i + 10] * inv, acc[i + 11] * inv);
+          w.w = pack_e4m3(acc[i + 12] * inv, acc[i + 13] * inv, acc[i + 14] * inv, acc[i + 15] * inv);
+          *reinterpret_cast<uint4*>(o + i) = w;
+        }
+        continue;
+      }
+      const int64_t o = row * a.out_srow + col0;
+#pragma unroll
+      for (int i = 0; i < 128; i += 8) {
+        if (a.wide && col0 + i + 8 <= a.N) {
+          if (a.out_dtype == XDIT_F32) {
+            float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + i);
+            d[0] = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+            d[1] = make_float4(acc[i + 4], acc[i + 5], acc[i + 6], acc[i + 7]);
+          } else {
+            uint4 w;
+            uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (a.out_dtype == XDIT_BF16) {
+                __nv_bfloat162 v = __floats2bfloat162_rn(acc[i + 2 * j], acc[i + 2 * j + 1]);
+                u[j] = *reinterpret_cast<uint32_t*>(&v);
+              } else {
+                __half2 v = __floats2half2_rn(acc[i + 2 * j], acc[i + 2 * j + 1]);
+                u[j] = *reinterpret_cast<uint32_t*>(&v);
+              }
+            }
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + o + i) = w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (col0 + i + j < a.N) store_any(a.out, a.out_dtype, o + i + j, acc[i + j]);
+        }
+      }
+    }
+  }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+  }
+  if (threadIdx.x == 0 && *abort_flag > 0) {
+    if (a.status) atomicCAS(a.status, 0, *abort_flag);
+    if (a.status_host) {  // host-visible copy, read by the next call without a synchronise
+      *reinterpret_cast<volatile int32_t*>(a.status_host) = *abort_flag;
+      __threadfence_system();
+    }
+  }
+}
+
+// Map of a row-major e4m3 matrix: a box is 128 bytes of K by `box_rows` rows; what lies outside reads as zero.
+int encode_rows(CUtensorMap* tm, const void* p, int64_t rows, int64_t K, int64_t stride, int box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return XDIT_E_DRIVER; }
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? stride : (K + 15) / 16 * 16)};  // a single row is never stepped
+  cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult %d (%lld x %lld, stride %lld)", (int)r, (long long)rows,
+              (long long)K, (long long)stride);
+    return XDIT_E_DRIVER;
+  }
+  return XDIT_OK;
+}
+
+// The attribute is per device; set once per device, under a lock (calls may come from several threads).
+template <auto Kernel>
+int configure_smem(int bytes) {
+  static std::mutex mu;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lk(mu);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return cuda_fail(e, "fp8 linear smem attribute");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  return XDIT_OK;
+}
+
+}  // namespace
+}  // namespace xdit
+
+using namespace xdit;
+
+extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* stream) {
+  const char* who = "xdit_fp8_linear";
+  if (!p) { set_error("%s: NULL params", who); return XDIT_E_NULL; }
+  if (p->M < 0 || p->N < 1 || p->K < 16 || p->K % 16 || (p->out_q && p->N % 16)) {
+    set_error("%s: M=%d N=%d K=%d (K a multiple of 16; N too where the result is e4m3 rows)", who, p->M, p->N, p->K);
+    return XDIT_E_SHAPE;
+  }
+  if (p->activation != XDIT_ACT_NONE && p->activation != XDIT_ACT_GELU_TANH) { set_error("%s: unknown activation %d", who, p->activation); return XDIT_E_DTYPE; }
+  const int es = p->out_q ? 1 : dtype_size(p->out_dtype);
+  if (!es || (p->bias && !dtype_size(p->bias_dtype))) { set_error("%s: bad dtype of the result (%d) or bias (%d)", who, p->out_dtype, p->bias_dtype); return XDIT_E_DTYPE; }
+  if (p->M == 0) return XDIT_OK;
+  if (!p->x || !p->x_scale || !p->w || !p->w_scale || (!p->out && !p->out_q) || (p->out_q && !p->out_scale)) { set_error("%s: NULL pointer", who); return XDIT_E_NULL; }
+  if ((((uintptr_t)p->x) & 15) || (((uintptr_t)p->w) & 15) || (p->M > 1 && (p->x_stride_row % 16 || p->x_stride_row < p->K)) ||
+      (p->N > 1 && (p->w_stride_row % 16 || p->w_stride_row < p->K)) || (p->out_q && ((((uintptr_t)p->out_q) & 15) || p->out_scale_ld < p->M))) {
+    set_error("%s: rows of x, w and out_q must start on 16-byte boundaries, out_scale_ld be at least M", who);
+    return XDIT_E_ALIGN;
+  }
+  if (!p->out_q && (((uintptr_t)p->out) % es || (p->M > 1 && p->out_stride_row < p->N))) { set_error("%s: out pointer or row stride", who); return XDIT_E_ALIGN; }
+  if (p->status_host) {
+    const int32_t code = *reinterpret_cast<const volatile int32_t*>(p->status_host);
+    if (code != 0) {
+      set_error("%s: an earlier launch gave up a bounded wait (code %d); nothing is launched until the status words "
+                "are cleared", who, code);
+      return XDIT_E_KERNEL_TIMEOUT;
+    }
+  }
+  int sms = 0;
+  int rc = check_device(&sms);
+  if (rc) return rc;
+  GemmArgs a;
+  memset(&a, 0, sizeof(a));
+  if ((rc = encode_rows(&a.tm_x, p->x, p->M, p->K, p->x_stride_row, kBM))) return rc;
+  if ((rc = encode_rows(&a.tm_w, p->w, p->N, p->K, p->w_stride_row, kBN))) return rc;
+  a.M = p->M; a.N = p->N;
+  a.kb = (p->K + kBK - 1) / kBK;
+  a.mt = (p->M + kBM - 1) / kBM;
+  a.nt = (p->N + kBN - 1) / kBN;
+  a.xs = p->x_scale; a.xs_srow = p->x_scale_stride_row; a.xs_skb = p->x_scale_stride_block;
+  a.ws = p->w_scale; a.ws_snb = p->w_scale_stride_row; a.ws_skb = p->w_scale_stride_block;
+  a.bias = p->bias; a.bias_dtype = p->bias_dtype; a.act = p->activation; a.out_dtype = p->out_dtype;
+  a.out = p->out; a.out_srow = p->out_stride_row;
+  a.out_q = (uint8_t*)p->out_q; a.out_scale = p->out_scale; a.out_scale_ld = p->out_scale_ld;
+  a.wide = ((uintptr_t)p->out) % 16 == 0 && (p->M == 1 || (p->out_stride_row * es) % 16 == 0);
+  a.status = p->status; a.status_host = p->status_host;
+  a.wait_limit_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
+  const int64_t tiles = (int64_t)a.mt * a.nt;
+  if (tiles > 0x3fffffffll) { set_error("%s: too many tiles", who); return XDIT_E_SHAPE; }
+  if ((rc = configure_smem<fp8_gemm_kernel>(kSmem))) return rc;
+  fp8_gemm_kernel<<<(int)(tiles < sms ? tiles : sms), kThreads, kSmem, (cudaStream_t)stream>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_kernel launch");
+  return XDIT_OK;
+}

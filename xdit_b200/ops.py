@@ -576,5 +576,282 @@ def qk_norm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: 
     launch_count += 1
 
 
+def _refuse_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("backward passes are not part of this inference path: call it under "
+                                  "torch.no_grad(), or with tensors that do not require a gradient")
+
+
+def _one_device(first: torch.Tensor, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+
+
+def _rows_contiguous(t: torch.Tensor, name: str) -> None:
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+
+
+_POSITIONS = {torch.int32: _capi.XDIT_POS_I32, torch.int64: _capi.XDIT_POS_I64, torch.float32: _capi.XDIT_POS_F32}
+
+
+def rotary_positions(frequencies, axis, axes: int, *, positions: Optional[torch.Tensor] = None,
+                     grid: Optional[Sequence[int]] = None, start: int = 0, batch: int = 1,
+                     rows: int = 0) -> _capi.RotaryPositions:
+    """Positions and angles as the rotary kernels take them.  ``frequencies`` and ``axis`` are ctypes arrays
+    (double, uint8) with one entry for each rotated pair.  ``positions``: int32, int64 or fp32, ``[rows, axes]`` or
+    ``[batch or 1, rows, axes]``; or ``grid``, the sides of a grid that the token index ``start + row`` walks."""
+    p = _capi.RotaryPositions(axes=axes, pairs=len(frequencies), frequencies=frequencies, axis=axis)
+    if (positions is None) == (grid is None):
+        raise ValueError("give either positions or a grid")
+    if grid is not None:
+        if len(grid) != axes or not 1 <= axes <= _capi.XDIT_ROTARY_MAX_AXES:
+            raise ValueError(f"a grid of {len(grid)} sides for {axes} axes (1..{_capi.XDIT_ROTARY_MAX_AXES})")
+        p.kind, p.start = _capi.XDIT_POS_GRID, int(start)
+        for i, side in enumerate(grid):
+            p.grid[i] = int(side)
+        return p
+    if positions.dtype not in _POSITIONS:
+        raise TypeError(f"positions must be int32, int64 or fp32, not {positions.dtype}")
+    t = positions if positions.dim() == 3 else positions.unsqueeze(0)
+    if t.dim() != 3 or t.shape[0] not in (1, batch) or t.shape[1] != rows or t.shape[2] != axes:
+        raise ValueError(f"positions {tuple(positions.shape)} for {batch} samples of {rows} tokens on {axes} axes")
+    p.kind, p.positions = _POSITIONS[t.dtype], t.data_ptr()
+    p.stride_b = t.stride(0) if t.shape[0] > 1 else 0
+    p.stride_row, p.stride_axis = t.stride(1), t.stride(2)
+    return p
+
+
+def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.RotaryPositions, halves: bool,
+                out_q: torch.Tensor, out_k: Optional[torch.Tensor]) -> None:
+    """Rotate ``q`` [B, H, s, D] and ``k`` [B, Hk, s, D] by the angles of ``positions`` (:func:`rotary_positions`) into
+    ``out_q`` and ``out_k``, which may be ``q`` and ``k`` themselves (``xdit_rotary_axes``)."""
+    global launch_count
+    p = _capi.RotaryParams(dtype=_dtype(q), halves=int(bool(halves)), pos=positions)
+    p.B, p.H, p.s, p.D = q.shape
+    p.q, p.out_q = q.data_ptr(), out_q.data_ptr()
+    pairs = [(q, out_q, "q")]
+    if k is not None:
+        p.Hk = k.shape[1]
+        p.k, p.out_k = k.data_ptr(), out_k.data_ptr()
+        pairs.append((k, out_k, "k"))
+    for i, (t, o, name) in enumerate(pairs):
+        if t.dtype != q.dtype or o.dtype != q.dtype:
+            raise TypeError("q, k and their outputs must share one dtype")
+        if o.shape != t.shape or t.shape[0] != p.B or t.shape[2] != p.s or t.shape[3] != p.D:
+            raise ValueError("q, k and their outputs must agree in B, s and D")
+        _rows_contiguous(t, name)
+        _rows_contiguous(o, "out_" + name)
+        p.stride_b[i], p.stride_h[i], p.stride_row[i] = t.stride(0), t.stride(1), t.stride(2)
+        p.out_stride_b[i], p.out_stride_h[i], p.out_stride_row[i] = o.stride(0), o.stride(1), o.stride(2)
+    if 2 * positions.pairs > p.D:
+        raise ValueError(f"{2 * positions.pairs} elements to rotate in a head of {p.D}")
+    _refuse_grad(q, k)
+    _require_cuda(q, k, out_q, out_k)
+    _one_device(q, k, out_q, out_k)
+    with torch.cuda.device(q.device):
+        _capi.check(_capi.load().xdit_rotary_axes(C.byref(p), _stream(q)), "xdit_rotary_axes")
+    launch_count += 1
+
+
+def rotary_tables(positions: _capi.RotaryPositions, s: int, D: int, device) -> tuple:
+    """``(cos, sin)``, fp32 ``[s, D]``, of the interleaved pairs at ``positions``: the tables that
+    :func:`qk_norm_rope_pack` takes (``xdit_rotary_tables``)."""
+    global launch_count
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise RuntimeError(f"xdit_b200 kernels run on CUDA devices only (sm_100a), not on {device}. There is no CPU fallback.")
+    cos, sin = (torch.empty(s, D, dtype=torch.float32, device=device) for _ in range(2))
+    with torch.cuda.device(device):
+        _capi.check(_capi.load().xdit_rotary_tables(C.byref(positions), cos.data_ptr(), sin.data_ptr(), s, D,
+                                                    _stream(cos)), "xdit_rotary_tables")
+    launch_count += 1
+    return cos, sin
+
+
+_NORMS = {None: _capi.XDIT_NORM_NONE, "layer": _capi.XDIT_NORM_LAYER, "rms": _capi.XDIT_NORM_RMS}
+
+
+def _row_vec(t: Optional[torch.Tensor], x: torch.Tensor, name: str, shared: bool = False) -> _capi.RowVec:
+    """A modulation row of ``x`` [B, s, C]: ``[C]``, ``[B or 1, C]`` or ``[B or 1, s or 1, C]``."""
+    if t is None:
+        return _capi.RowVec()
+    B, s, Cn = x.shape
+    if t.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{name} must be {x.dtype} or fp32, not {t.dtype}")
+    shape = t.shape if t.dim() == 3 else (t.shape[0], 1, t.shape[1]) if t.dim() == 2 else (1, 1) + tuple(t.shape)
+    if len(shape) != 3 or shape[0] not in (1, B) or shape[1] not in (1, s) or shape[2] != Cn or (shared and t.dim() != 1):
+        raise ValueError(f"{name} of shape {tuple(t.shape)} for rows of shape {tuple(x.shape)}")
+    _rows_contiguous(t, name)
+    v = _capi.RowVec(ptr=t.data_ptr(), dtype=_dtype(t))
+    v.stride_b = t.stride(0) if t.dim() > 1 and shape[0] > 1 else 0
+    v.stride_row = t.stride(1) if t.dim() == 3 and shape[1] > 1 else 0
+    return v
+
+
+def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], *, out_residual=None, out=None,
+                        out_q=None, out_scale=None, gate=None, residual_scale: float = 1.0, post_norm=None,
+                        post_weight=None, post_bias=None, norm=None, weight=None, bias=None, scale=None, shift=None,
+                        eps: float = 1e-6) -> None:
+    """``out_residual = residual_scale * residual + gate * post_norm(branch)`` and ``out = norm(that) * (1 + scale) +
+    shift`` in one launch (``xdit_gated_residual_norm``); all ``[B, s, C]``.  ``out_q`` (e4m3 ``[B*s, C]``) with ``out_scale``
+    (fp32 ``[B*s, C/128]``, stored block by block) takes the second result quantised instead of ``out``."""
+    global launch_count
+    if residual.dim() != 3:
+        raise ValueError("expected [B, s, C]")
+    if norm not in _NORMS or post_norm not in _NORMS:
+        raise ValueError("a norm is None, 'layer' or 'rms'")
+    if norm is None and any(t is not None for t in (weight, bias, scale, shift)):
+        raise ValueError("weight, bias, scale and shift need a norm")
+    if branch is None and (post_norm is not None or gate is not None):
+        raise ValueError("gate and post_norm need a branch")
+    if post_norm is None and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight and post_bias need a post_norm")
+    p = _capi.NormParams(dtype=_dtype(residual), post_norm=_NORMS[post_norm], norm=_NORMS[norm],
+                         residual_scale=float(residual_scale), eps=float(eps))
+    p.B, p.s, p.C = residual.shape
+    for name, t in (("residual", residual), ("branch", branch), ("out_residual", out_residual), ("out", out)):
+        if t is None:
+            continue
+        if t.shape != residual.shape:
+            raise ValueError(f"{name} {tuple(t.shape)} beside a residual {tuple(residual.shape)}")
+        if t.dtype != residual.dtype:
+            raise TypeError(f"{name} must have the residual's dtype")
+        _rows_contiguous(t, name)
+        setattr(p, name, t.data_ptr())
+        setattr(p, name + "_stride_b", t.stride(0))
+        setattr(p, name + "_stride_row", t.stride(1))
+    if out_q is not None:
+        p.out_q, p.out_scale, p.out_scale_ld = out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)):
+        if t is not None:
+            setattr(p, name, _row_vec(t, residual, name, shared=True))
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is not None:
+            setattr(p, name, _row_vec(t, residual, name))
+    every = (branch, out_residual, out, out_q, out_scale, gate, post_weight, post_bias, weight, bias, scale, shift)
+    _refuse_grad(residual, *every)
+    _require_cuda(residual, *every)
+    _one_device(residual, *every)
+    with torch.cuda.device(residual.device):
+        _capi.check(_capi.load().xdit_gated_residual_norm(C.byref(p), _stream(residual)), "xdit_gated_residual_norm")
+    launch_count += 1
+
+
+def _scale_ld(scale: torch.Tensor) -> int:
+    """Distance between two blocks' scales of row scales [rows, blocks] that are stored block by block."""
+    if scale.shape[0] > 1 and scale.stride(0) != 1:
+        raise ValueError("row scales are written block by block: scale.stride(0) must be 1")
+    return scale.stride(1) if scale.shape[1] > 1 else max(1, scale.shape[0])
+
+
+def empty_fp8_rows(rows: int, K: int, device) -> tuple:
+    """``(data, scale)`` for ``rows`` e4m3 rows of ``K`` values: uint8-sized ``[rows, K]`` and fp32 ``[rows, K/128]`` whose blocks
+    lie behind one another, as the kernels write and read them."""
+    data = torch.empty(rows, K, dtype=torch.float8_e4m3fn, device=device)
+    kb = -(-K // _capi.XDIT_FP8_BLOCK)
+    return data, torch.empty(kb, rows, dtype=torch.float32, device=device).t()
+
+
+def quantize_rows(x: torch.Tensor) -> tuple:
+    """``x`` [B, s, K] -> ``(data, scale)``: e4m3 ``[B*s, K]`` with a power-of-two scale for each block of 128 of a row
+    (``xdit_quantize_rows``)."""
+    global launch_count
+    if x.dim() != 3:
+        raise ValueError("expected [B, s, K]")
+    B, s, K = x.shape
+    if K % 16 or K == 0:
+        raise ValueError(f"rows of {K} values: a multiple of 16 is needed")
+    dt = _dtype(x)
+    _rows_contiguous(x, "x")
+    _refuse_grad(x)
+    _require_cuda(x)
+    data, scale = empty_fp8_rows(B * s, K, x.device)
+    with torch.cuda.device(x.device):
+        _capi.check(_capi.load().xdit_quantize_rows(x.data_ptr(), x.stride(0), x.stride(1), dt, B, s, K,
+                                                    data.data_ptr(), scale.data_ptr(), _scale_ld(scale), _stream(x)),
+                    "xdit_quantize_rows")
+    launch_count += 1
+    return data, scale
+
+
+def quantize_weight(w: torch.Tensor) -> tuple:
+    """``w`` [N, K] -> ``(data, scale)``: e4m3 ``[N, K]`` with a power-of-two scale for each block of 128 x 128
+    (``xdit_quantize_weight``)."""
+    global launch_count
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 16 or w.shape[1] % 16:
+        raise ValueError(f"a weight [N, K] with K a multiple of 16 is needed, got {tuple(w.shape)}")
+    dt = _dtype(w)
+    _rows_contiguous(w, "w")
+    _refuse_grad(w)
+    _require_cuda(w)
+    N, K = w.shape
+    data = torch.empty(N, K, dtype=torch.float8_e4m3fn, device=w.device)
+    b = _capi.XDIT_FP8_BLOCK
+    scale = torch.empty(-(-N // b), -(-K // b), dtype=torch.float32, device=w.device)
+    with torch.cuda.device(w.device):
+        _capi.check(_capi.load().xdit_quantize_weight(w.data_ptr(), w.stride(0), dt, N, K, data.data_ptr(),
+                                                      scale.data_ptr(), _stream(w)), "xdit_quantize_weight")
+    launch_count += 1
+    return data, scale
+
+
+_ACTIVATIONS = {None: _capi.XDIT_ACT_NONE, "gelu_tanh": _capi.XDIT_ACT_GELU_TANH}
+
+
+def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
+               out: Optional[torch.Tensor] = None, out_q: Optional[torch.Tensor] = None,
+               out_scale: Optional[torch.Tensor] = None, _wait_limit_ns: int = 0) -> None:
+    """``out = act(x w^T + bias)`` of e4m3 rows ``x`` [M, K] and a weight ``w`` [N, K] with fp32 scales ``x_scale`` [M, K/128] and
+    ``w_scale`` [N/128, K/128] of any value and strides (``xdit_fp8_linear``).  ``out`` [M, N] in bf16, fp16 or fp32, or ``out_q``
+    with ``out_scale`` for e4m3 rows again."""
+    global launch_count
+    b = _capi.XDIT_FP8_BLOCK
+    if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
+        raise TypeError("x and w must be float8_e4m3fn")
+    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise TypeError("the scales must be fp32")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"rows {tuple(x.shape)} and a weight {tuple(w.shape)}")
+    M, K = x.shape
+    N = w.shape[0]
+    if K % 16 or K == 0 or N == 0:
+        raise ValueError(f"K = {K}: a multiple of 16 is needed (and N = {N} rows of the weight)")
+    if tuple(x_scale.shape) != (M, -(-K // b)) or tuple(w_scale.shape) != (-(-N // b), -(-K // b)):
+        raise ValueError(f"scales {tuple(x_scale.shape)} and {tuple(w_scale.shape)} for rows {tuple(x.shape)} and a weight {tuple(w.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError("an activation is None or 'gelu_tanh'")
+    if bias is not None and (tuple(bias.shape) != (N,) or (bias.stride(0) != 1 and N > 1)):
+        raise ValueError(f"a contiguous bias of {N} values is needed")
+    if (out is None) == (out_q is None):
+        raise ValueError("give either out or out_q")
+    p = _capi.Fp8LinearParams(M=M, N=N, K=K, activation=_ACTIVATIONS[activation])
+    if out is not None:
+        if tuple(out.shape) != (M, N):
+            raise ValueError(f"out {tuple(out.shape)} for a result of {(M, N)}")
+        _rows_contiguous(out, "out")
+        p.out_dtype, p.out, p.out_stride_row = _dtype(out), out.data_ptr(), out.stride(0)
+    else:
+        if N % 16:
+            raise ValueError(f"e4m3 rows of {N} values: a multiple of 16 is needed")
+        p.out_q, p.out_scale, p.out_scale_ld = out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)
+    for t, name in ((x, "x"), (w, "w")):
+        _rows_contiguous(t, name)
+    p.x, p.x_stride_row, p.w, p.w_stride_row = x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0)
+    p.x_scale, p.x_scale_stride_row, p.x_scale_stride_block = x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1)
+    p.w_scale, p.w_scale_stride_row, p.w_scale_stride_block = w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1)
+    if bias is not None:
+        p.bias, p.bias_dtype = bias.data_ptr(), _dtype(bias)
+    _refuse_grad(bias)
+    _require_cuda(x, x_scale, w, w_scale, bias, out, out_q, out_scale)
+    _one_device(x, x_scale, w, w_scale, bias, out, out_q, out_scale)
+    st = _status(x.device)
+    p.status, p.status_host, p.wait_limit_ns = st.dev.data_ptr(), st.host.data_ptr(), int(_wait_limit_ns)
+    _launch_attn(_capi.load().xdit_fp8_linear, p, x, "xdit_fp8_linear")
+    launch_count += 1
+
+
 def default_scale(D: int) -> float:
     return 1.0 / math.sqrt(D)

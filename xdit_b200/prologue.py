@@ -18,7 +18,7 @@ processor defines inline.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.distributed as dist
@@ -27,19 +27,20 @@ from . import ops
 from . import usp as _usp
 from .distributed import (PROCESS_GROUP, get_ring_parallel_world_size, get_ulysses_parallel_rank,
                           get_ulysses_parallel_world_size)
+from .rotary import RotaryEmbedding
 
 
 def qk_norm_rope_heads(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, heads: int, *,
                        norm_q_weight: Optional[torch.Tensor] = None, norm_k_weight: Optional[torch.Tensor] = None,
                        eps: float = 1e-6, norm_per_head: bool = False,
-                       rotary_emb: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                       rotary_emb: Union[RotaryEmbedding, Tuple[torch.Tensor, torch.Tensor], None] = None
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Projections ``[B, s, heads*D]`` -> normalised, rotated ``q, k`` and ``v`` as ``[B, heads, s, D]``
     tensors (what the processor passes to ``USP``).  One launch; for ``B > 1`` the results are
     ``[heads, B, s, D]`` buffers viewed with the batch axis first."""
     B, s, HD = query.shape
     D = HD // heads
-    cos, sin = _cos_sin(rotary_emb, s, D)
+    cos, sin = _cos_sin(rotary_emb, s, D, query.device)
     n = heads * B * s * D
     buf = torch.empty(3 * n, dtype=query.dtype, device=query.device)
     ops.qk_norm_rope_pack(query, key, value, heads, buf, buf[n:], buf[2 * n:], (n, n, n), 1,
@@ -48,9 +49,11 @@ def qk_norm_rope_heads(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     return tuple(buf[i * n:(i + 1) * n].view(heads, B, s, D).permute(1, 0, 2, 3) for i in range(3))
 
 
-def _cos_sin(rotary_emb, s, D):
+def _cos_sin(rotary_emb, s, D, device):
     if rotary_emb is None:
         return None, None
+    if isinstance(rotary_emb, RotaryEmbedding):
+        return rotary_emb.tables(s, D, device)
     cos, sin = rotary_emb
     # the processors carry [1, s, 1, D] tables (transformer_wan.py:108-120); [s, D] is accepted as well
     cos = cos.reshape(s, D) if cos.numel() == s * D else cos
@@ -64,7 +67,7 @@ def attention_from_projections(query: torch.Tensor, key: torch.Tensor, value: to
                                norm_q_weight: Optional[torch.Tensor] = None,
                                norm_k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
                                norm_per_head: bool = False,
-                               rotary_emb: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                               rotary_emb: Union[RotaryEmbedding, Tuple[torch.Tensor, torch.Tensor], None] = None,
                                softmax_scale: Optional[float] = None,
                                out_proj_weight: Optional[torch.Tensor] = None,
                                out_proj_bias: Optional[torch.Tensor] = None, attn_layer=None) -> torch.Tensor:
@@ -106,7 +109,7 @@ def _attention_with_stale_kv(query, key, value, heads, norm_q_weight, norm_k_wei
     D = HD // heads
     kc, vc, start = get_cache_manager().rows_for_producer(attn_layer, B, heads, n, D, query.dtype, query.device)
     S = kc.shape[2]
-    cos, sin = _cos_sin(rotary_emb, n, D)
+    cos, sin = _cos_sin(rotary_emb, n, D, query.device)
     q_buf = torch.empty(heads * B * n * D, dtype=query.dtype, device=query.device)
     # q in the packed [H][B][n][D] layout; k and v rows at [start, start + n) of the [B,H,S,D] buffers
     ops.qk_norm_rope_pack(query, key, value, heads, q_buf, kc.view(-1)[start * D:], vc.view(-1)[start * D:],
@@ -145,7 +148,7 @@ def _attention_from_projections(query, key, value, heads, norm_q_weight, norm_k_
         return out.permute(0, 2, 1, 3).reshape(B, s, HD)
     assert heads % U == 0, "h must be divisible by world_size, got {} and {}".format(heads, U)
     Hl = heads // U
-    cos, sin = _cos_sin(rotary_emb, s, D)
+    cos, sin = _cos_sin(rotary_emb, s, D, query.device)
     blk = Hl * B * s * D
     stride = 3 * blk
     send = torch.empty(U * stride, dtype=query.dtype, device=query.device)
