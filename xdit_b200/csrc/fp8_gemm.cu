@@ -6,13 +6,17 @@
 //
 // One CTA per SM walks output tiles of 128 rows x 256 columns.  A step is one block of 128 along K, which
 // is also one 128-byte swizzle row of the operands in shared memory:
-//   warp 9     loads the step's operands by TMA (16 KB of x, 32 KB of W) into a ring
-//   warp 8     issues the step's four MMAs (128 x 256 x 32) into one of two TMEM buffers of 256 columns
-//   warps 0-7  two warpgroups, 128 columns each: thread = row, 128 fp32 sums in registers; they add the
-//              scaled buffer of one step while the tensor core fills the other
-// A warpgroup's columns share ws, so the scale of a step is one product per thread.  After the last step the
-// sums get bias and activation and are written, rounded once; or they become e4m3 rows again: a
-// thread holds a whole block of 128 of its row, so that block's scale needs no exchange.
+//   warp 17      loads the step's operands by TMA (16 KB of x, 32 KB of W) into a ring
+//   warp 18      copies the step's scales (128 of x, 2 of W) into a ring of their own, up to 16 steps ahead: read
+//                when they are needed, they arrived later than the MMAs (780 against 705 cycles a step)
+//   warp 16      issues the step's four MMAs (128 x 256 x 32) into one of two TMEM buffers of 256 columns
+//   warps 0-15   four warpgroups, 64 columns each: thread = row, 64 fp32 sums in registers; they add the scaled
+//                buffer of one step while the tensor core fills the other.  Four warps a scheduler keep its FMA
+//                pipe busier than two with 128 sums each (705 against 810 cycles); the MMAs alone take 595.
+// After the last step the sums get bias and activation and are rounded once; they leave through shared memory and
+// TMA stores, which also clip the edges (16-byte stores from registers, 32 rows an instruction, cost a fifth of
+// the whole time).  Or they become e4m3 rows again: two warpgroups hold a block of 128 and exchange the rows'
+// largest magnitudes.
 //
 // Every wait on an mbarrier is bounded in time; when one gives up the CTA raises a flag in shared memory, all
 // roles leave their loops, outstanding copies and MMAs are drained with bounded waits, TMEM is freed and
@@ -26,18 +30,27 @@
 namespace xdit {
 namespace {
 
-constexpr int kThreads = 384;  // 8 summing warps, MMA warp, TMA warp, 2 idle warps (full register-trading warpgroup)
+constexpr int kThreads = 640;  // 16 summing warps, MMA warp, TMA warp, scale warp, 1 idle warp (full register-trading warpgroup)
 constexpr int kBM = 128, kBN = 256, kBK = XDIT_FP8_BLOCK;
-constexpr int kStages = 4;
+constexpr int kCols = 64;      // columns of a summing thread
+constexpr int kStages = 3;
+constexpr int kAhead = 16;     // steps whose scales are in shared memory or on their way
 constexpr int kABytes = kBM * kBK, kBBytes = kBN * kBK, kStageBytes = kABytes + kBBytes;
-constexpr int kBarOff = kStages * kStageBytes;
-constexpr int kNumBars = 2 * kStages + 4 + 1;
+constexpr int kWarpOut = 32 * kCols * 2;                // staging of a summing warp's results
+constexpr int kOutOff = kStages * kStageBytes;
+constexpr int kBiasOff = kOutOff + 16 * kWarpOut;       // [16 warps][64 columns]
+constexpr int kScaleOff = kBiasOff + 16 * kCols * 4;    // [kAhead][128 rows of x + 2 of w, padded]
+constexpr int kScaleBytes = 576;
+constexpr int kTopOff = kScaleOff + kAhead * kScaleBytes;  // [2 turns][4 warpgroups][128 rows] largest magnitudes
+constexpr int kBarOff = kTopOff + 2 * 4 * 128 * 4;
+constexpr int kGroup = 4, kGroups = kAhead / kGroup;  // steps whose scales share a barrier
+constexpr int kNumBars = 2 * kStages + 4 + 1 + 2 * kGroups + 2;
 constexpr int kMiscOff = kBarOff + kNumBars * 8;
 constexpr int kSmem = kMiscOff + 16 + 1024;  // with slack to align the base to 1024 bytes
 constexpr int kBand = 16;                    // row tiles of a band: tiles of a band are walked column by column
 
 struct alignas(64) GemmArgs {
-  CUtensorMap tm_x, tm_w;
+  CUtensorMap tm_x, tm_w, tm_out;
   int32_t M, N, kb;        // kb: blocks along K
   int32_t mt, nt;          // tiles
   const float* xs;
@@ -52,6 +65,7 @@ struct alignas(64) GemmArgs {
   float* out_scale;
   int64_t out_scale_ld;
   int32_t wide;            // 16-byte stores are possible
+  int32_t tma_out;         // the results leave through shared memory and tm_out
   int32_t* status;
   int32_t* status_host;
   uint32_t wait_limit_ns;
@@ -61,6 +75,25 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tm), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// acc += s * p for the pair of columns (acc0, acc1)
+__device__ __forceinline__ void fma_pair(float& acc0, float& acc1, uint32_t p0, uint32_t p1, uint64_t s2) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tfma.rn.f32x2 x, y, %4, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(acc0), "+f"(acc1) : "r"(p0), "r"(p1), "l"(s2));
+}
+__device__ __forceinline__ uint32_t pack16(int dtype, float lo, float hi) {
+  if (dtype == XDIT_BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
 }
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -100,6 +133,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
   auto bar_tfull = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
   auto bar_tempty = [&](int s) { return bar0 + 8u * (2 * kStages + 2 + s); };
   const uint32_t bar_drain = bar0 + 8u * (2 * kStages + 4);
+  auto bar_sfull = [&](int s) { return bar0 + 8u * (2 * kStages + 5 + s); };
+  auto bar_sempty = [&](int s) { return bar0 + 8u * (2 * kStages + 5 + kGroups + s); };
+  auto bar_top = [&](int pair) { return bar0 + 8u * (2 * kStages + 5 + 2 * kGroups + pair); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + kMiscOff + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -107,12 +143,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(bar_tfull(s), 1); mbar_init(bar_tempty(s), 256); }
+    for (int s = 0; s < 2; ++s) { mbar_init(bar_tfull(s), 1); mbar_init(bar_tempty(s), 16); }
+    for (int s = 0; s < kGroups; ++s) { mbar_init(bar_sfull(s), 32); mbar_init(bar_sempty(s), 16); }
+    for (int s = 0; s < 2; ++s) mbar_init(bar_top(s), 8);
     mbar_init(bar_drain, 1);
     *abort_flag = status_is_set(a.status) ? -1 : 0;  // -1: skip all work (an earlier failure is pending)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -124,9 +162,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 
   if (skip) {
     // nothing to do: fall through to the teardown, which frees TMEM
-  } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");  // 2 x 232 + 40 <= 512 per scheduler
-    if (warp == 9) {
+  } else if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");  // per scheduler 4 x 112 + 32 = 5 x 96, what the launch holds
+    if (warp == 17) {
       // ======================= TMA producer =======================
       if (lane == 0) {
         int issued = 0;
@@ -150,7 +188,42 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_full(i % kStages), (i / kStages) & 1); ++it) __nanosleep(64);
         }
       }
-    } else if (warp == 8) {
+    } else if (warp == 18) {
+      // ======================= scales: each lane the rows lane, lane + 32, ... of the tile =======================
+      // A load from L2 takes longer than a step, so they are copied asynchronously, up to kAhead steps ahead.
+      int step = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int m, n;
+        tile_at(a, t, m, n);
+        const float* src[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = m * kBM + 32 * i + lane;  // rows and columns behind the end take any scale
+          src[i] = a.xs + (int64_t)(row < a.M ? row : 0) * a.xs_srow;
+        }
+        const int nb = n * (kBN / kBK) + (lane & 1);
+        const float* w = a.ws + (int64_t)(nb * kBK < a.N ? nb : 0) * a.ws_snb;
+        for (int c = 0; c < a.kb; ++c, ++step) {
+          const int slot = step % kAhead, turn = step / kAhead, group = slot / kGroup;
+          if (turn > 0 && step % kGroup == 0) ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty(group), (turn - 1) & 1, abort_flag, a.wait_limit_ns, 320));
+          if (!ok) break;
+          const uint32_t at = base + kScaleOff + slot * kScaleBytes + lane * 4;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 128 * i), "l"(src[i]) : "memory");
+            src[i] += a.xs_skb;
+          }
+          if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 512), "l"(w) : "memory");
+          w += a.ws_skb;
+          if (step % kGroup == kGroup - 1)
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_sfull(group)) : "memory");
+        }
+      }
+      if (step % kGroup)  // the last group is not full
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_sfull(step % kAhead / kGroup)) : "memory");
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == 16) {
       // ======================= MMA issuer (the warp runs converged, one elected lane issues) =======================
       const bool leader = elect_one();
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
@@ -163,16 +236,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         for (int c = 0; c < a.kb; ++c, ++step) {
           const int st = step % kStages, buf = step & 1;
-          if (step >= 2) ok = wait_all(bar_tempty(buf), ((step >> 1) - 1) & 1, 200 + buf);
-          if (ok) ok = wait_all(bar_full(st), (step / kStages) & 1, 210 + st);
+          ok = wait_all(bar_full(st), (step / kStages) & 1, 210 + st);
+          if (ok && step >= 2) ok = wait_all(bar_tempty(buf), ((step >> 1) - 1) & 1, 200 + buf);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
             const uint64_t da = desc_kmajor(base + st * kStageBytes), db = desc_kmajor(base + st * kStageBytes + kABytes);
 #pragma unroll
             for (int k = 0; k < kBK / 32; ++k) mma_f8(tmem_u + buf * kBN, da + 2 * k, db + 2 * k, idesc, k > 0);
-            tc_commit(bar_empty(st));
             tc_commit(bar_tfull(buf));
+            tc_commit(bar_empty(st));
           }
         }
       }
@@ -185,109 +258,143 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ======================= scaled sums + epilogue =======================
-    const int half = warp >> 2;  // columns [128 half, 128 half + 128) of the tile
-    const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
+    const int group = warp >> 2;  // columns [64 group, 64 group + 64) of the tile
+    const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * kCols;
     const int row_in = (warp & 3) * 32 + lane;
+    const uint32_t scale_x = base + kScaleOff + row_in * 4, scale_w = base + kScaleOff + 512 + (group >> 1) * 4;
+    const uint32_t stage = base + kOutOff + warp * kWarpOut;
+    float* bias = reinterpret_cast<float*>(base_ptr + kBiasOff) + warp * kCols;
+    float* tops = reinterpret_cast<float*>(base_ptr + kTopOff);
     bool ok = true;
-    int step = 0;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    int step = 0, turn = 0;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++turn) {
       int m, n;
       tile_at(a, t, m, n);
-      const int64_t row = (int64_t)m * kBM + row_in;
-      const int col0 = n * kBN + half * 128;
-      const bool live = row < a.M && col0 < a.N;
-      const float* xs = a.xs + (live ? row : 0) * a.xs_srow;
-      const float* ws = a.ws + (live ? col0 / kBK : 0) * a.ws_snb;
-      float acc[128];
+      const int row0 = m * kBM + (warp & 3) * 32, col0 = n * kBN + group * kCols;
+      if (a.bias) {
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-      float sx = __ldg(xs), sw = __ldg(ws);
+        for (int i = 0; i < kCols; i += 32)
+          bias[i + lane] = col0 + i + lane < a.N ? load_any(a.bias, a.bias_dtype, col0 + i + lane) : 0.f;
+        __syncwarp();
+      }
+      float acc[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) acc[i] = 0;
+#pragma unroll 1
       for (int c = 0; c < a.kb; ++c, ++step) {
-        const int buf = step & 1;
-        const float s = live ? sx * sw : 0.f;
-        if (c + 1 < a.kb) { sx = __ldg(xs + (c + 1) * a.xs_skb); sw = __ldg(ws + (c + 1) * a.ws_skb); }
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull(buf), (step >> 1) & 1, abort_flag, a.wait_limit_ns, 300 + buf));
-        if (!ok) break;
+        const int buf = step & 1, slot = step % kAhead;
+        // no way out of this loop: with one, the compiler copies all sums in every step.  After a wait that gave
+        // up, the others return at once.
+        if (step % kGroup == 0) ok &= mbar_wait(bar_sfull(slot / kGroup), (step / kAhead) & 1, abort_flag, a.wait_limit_ns, 310);
+        float sx, sw;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sx) : "r"(scale_x + slot * kScaleBytes) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sw) : "r"(scale_w + slot * kScaleBytes) : "memory");
+        const uint64_t s2 = f2_pack(sx * sw, sx * sw);
+        ok &= mbar_wait(bar_tfull(buf), (step >> 1) & 1, abort_flag, a.wait_limit_ns, 300 + buf);
+        __syncwarp();
         tc_fence_after();
+        const uint32_t tb = taddr + buf * kBN;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kCols / 32; ++q) {
           uint32_t p[32];
-          XDIT_TMEM_LD32(p, 0, taddr + buf * kBN + 32 * q);
+          XDIT_TMEM_LD32(p, 0, tb + 32 * q);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[32 * q + i] = fmaf(s, __uint_as_float(p[i]), acc[32 * q + i]);
+          for (int i = 0; i < 16; ++i)
+            fma_pair(acc[32 * q + 2 * i], acc[32 * q + 2 * i + 1], p[2 * i], p[2 * i + 1], s2);
         }
         tc_fence_before();
-        mbar_arrive(bar_tempty(buf));
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar_tempty(buf));
+          if (step % kGroup == kGroup - 1) mbar_arrive(bar_sempty(slot / kGroup));
+        }
       }
-      if (!ok || !live) continue;
+      ok = __all_sync(0xffffffffu, ok);
+      const int64_t row = row0 + lane;
+      const bool live = ok && row < a.M && col0 < a.N;
       if (a.bias) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (col0 + i < a.N) acc[i] += load_any(a.bias, a.bias_dtype, col0 + i);
+        for (int i = 0; i < kCols; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(bias + i);
+          acc[i] += v.x; acc[i + 1] += v.y; acc[i + 2] += v.z; acc[i + 3] += v.w;
+        }
       }
       if (a.act == XDIT_ACT_GELU_TANH) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) acc[i] = gelu_tanh(acc[i]);
+        for (int i = 0; i < kCols; ++i) acc[i] = gelu_tanh(acc[i]);
+      }
+      if (a.tma_out) {  // the last tile's results have left the staging buffer
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
       }
       if (a.out_q) {
+        // two warpgroups hold a block of 128 columns: they exchange their rows' largest magnitudes.  The buffer
+        // alternates, so the wait of one tile also keeps the next one's writes off it.
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
+        for (int i = 0; i < kCols; ++i)
           if (col0 + i < a.N) top = amax_nan(top, acc[i]);
+        float* buf = tops + (turn & 1) * 512;
+        buf[group * 128 + row_in] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_top(group >> 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_top(group >> 1), turn & 1, abort_flag, a.wait_limit_ns, 330));
+        top = amax_nan(top, buf[(group ^ 1) * 128 + row_in]);
         float inv;
-        a.out_scale[(col0 / kBlock) * a.out_scale_ld + row] = block_scale(top, inv);
-        uint8_t* o = a.out_q + row * a.N + col0;
+        const float sc = block_scale(top, inv);
+        if (live && !(group & 1)) a.out_scale[(col0 / kBlock) * a.out_scale_ld + row] = sc;
 #pragma unroll
-        for (int i = 0; i < 128; i += 16) {
-          if (col0 + i >= a.N) break;  // N is a multiple of 16 here
+        for (int i = 0; i < kCols; i += 16) {
           uint4 w;
           w.x = pack_e4m3(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
           w.y = pack_e4m3(acc[i + 4] * inv, acc[i + 5] * inv, acc[i + 6] * inv, acc[i + 7] * inv);
           w.z = pack_e4m3(acc[i + 8] * inv, acc[i + 9] * inv, acc[i + 10] * inv, acc[i + 11] * inv);
           w.w = pack_e4m3(acc[i + 12] * inv, acc[i + 13] * inv, acc[i + 14] * inv, acc[i + 15] * inv);
-          *reinterpret_cast<uint4*>(o + i) = w;
+          st_shared16(stage + lane * 64 + (((i >> 4) ^ ((lane >> 1) & 3)) << 4), w);  // 64-byte swizzle
         }
-        continue;
-      }
-      const int64_t o = row * a.out_srow + col0;
+      } else if (a.tma_out) {
 #pragma unroll
-      for (int i = 0; i < 128; i += 8) {
-        if (a.wide && col0 + i + 8 <= a.N) {
-          if (a.out_dtype == XDIT_F32) {
-            float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + i);
-            d[0] = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-            d[1] = make_float4(acc[i + 4], acc[i + 5], acc[i + 6], acc[i + 7]);
+        for (int i = 0; i < kCols; i += 8) {
+          uint4 w;
+          w.x = pack16(a.out_dtype, acc[i], acc[i + 1]);
+          w.y = pack16(a.out_dtype, acc[i + 2], acc[i + 3]);
+          w.z = pack16(a.out_dtype, acc[i + 4], acc[i + 5]);
+          w.w = pack16(a.out_dtype, acc[i + 6], acc[i + 7]);
+          st_shared16(stage + lane * 128 + (((i >> 3) ^ (lane & 7)) << 4), w);  // 128-byte swizzle
+        }
+      } else if (live) {
+        const int64_t o = row * a.out_srow + col0;
+#pragma unroll
+        for (int i = 0; i < kCols; i += 4) {
+          if (a.wide && a.out_dtype == XDIT_F32 && col0 + i + 4 <= a.N) {
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
           } else {
-            uint4 w;
-            uint32_t* u = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (a.out_dtype == XDIT_BF16) {
-                __nv_bfloat162 v = __floats2bfloat162_rn(acc[i + 2 * j], acc[i + 2 * j + 1]);
-                u[j] = *reinterpret_cast<uint32_t*>(&v);
-              } else {
-                __half2 v = __floats2half2_rn(acc[i + 2 * j], acc[i + 2 * j + 1]);
-                u[j] = *reinterpret_cast<uint32_t*>(&v);
-              }
-            }
-            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + o + i) = w;
+            for (int j = 0; j < 4; ++j)
+              if (col0 + i + j < a.N) store_any(a.out, a.out_dtype, o + i + j, acc[i + j]);
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (col0 + i + j < a.N) store_any(a.out, a.out_dtype, o + i + j, acc[i + j]);
+        }
+      }
+      if (a.tma_out) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && ok && row0 < a.M && col0 < a.N) {  // what lies behind the end of a row or column is not written
+          tma_store_2d(&a.tm_out, stage, col0, row0);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
     }
+    if (a.tma_out && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   // ---------------- teardown ----------------
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
   }
@@ -300,19 +407,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
   }
 }
 
-// Map of a row-major e4m3 matrix: a box is 128 bytes of K by `box_rows` rows; what lies outside reads as zero.
-int encode_rows(CUtensorMap* tm, const void* p, int64_t rows, int64_t K, int64_t stride, int box_rows) {
+// Map of a row-major matrix of `type`: boxes of `box_cols` by `box_rows`; what lies outside reads as zero and is not written.
+int encode_map(CUtensorMap* tm, CUtensorMapDataType type, int es, const void* p, int64_t rows, int64_t cols, int64_t stride,
+               int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return XDIT_E_DRIVER; }
-  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? stride : (K + 15) / 16 * 16)};  // a single row is never stepped
-  cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? stride * es : (cols * es + 15) / 16 * 16)};  // a single row is never stepped
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  CUresult r = fn(tm, type, 2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d (%lld x %lld, stride %lld)", (int)r, (long long)rows,
-              (long long)K, (long long)stride);
+              (long long)cols, (long long)stride);
     return XDIT_E_DRIVER;
   }
   return XDIT_OK;
@@ -371,8 +478,9 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   if (rc) return rc;
   GemmArgs a;
   memset(&a, 0, sizeof(a));
-  if ((rc = encode_rows(&a.tm_x, p->x, p->M, p->K, p->x_stride_row, kBM))) return rc;
-  if ((rc = encode_rows(&a.tm_w, p->w, p->N, p->K, p->w_stride_row, kBN))) return rc;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  if ((rc = encode_map(&a.tm_x, u8, 1, p->x, p->M, p->K, p->x_stride_row, kBM, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  if ((rc = encode_map(&a.tm_w, u8, 1, p->w, p->N, p->K, p->w_stride_row, kBN, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   a.M = p->M; a.N = p->N;
   a.kb = (p->K + kBK - 1) / kBK;
   a.mt = (p->M + kBM - 1) / kBM;
@@ -383,6 +491,12 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   a.out = p->out; a.out_srow = p->out_stride_row;
   a.out_q = (uint8_t*)p->out_q; a.out_scale = p->out_scale; a.out_scale_ld = p->out_scale_ld;
   a.wide = ((uintptr_t)p->out) % 16 == 0 && (p->M == 1 || (p->out_stride_row * es) % 16 == 0);
+  a.tma_out = p->out_q || (a.wide && es == 2);
+  if (p->out_q)
+    rc = encode_map(&a.tm_out, u8, 1, p->out_q, p->M, p->N, p->N, 32, kCols, CU_TENSOR_MAP_SWIZZLE_64B);
+  else if (a.tma_out)
+    rc = encode_map(&a.tm_out, u16, 2, p->out, p->M, p->N, p->out_stride_row, 32, kCols, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
   a.status = p->status; a.status_host = p->status_host;
   a.wait_limit_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
   const int64_t tiles = (int64_t)a.mt * a.nt;
