@@ -15,6 +15,8 @@
 namespace xdit {
 namespace {
 
+constexpr int kQuantThreads = 160;
+
 struct RowVec {  // a row of C values: the same for all, or with a stride for samples or tokens
   const void* ptr;
   int64_t stride_b, stride_row;
@@ -49,56 +51,139 @@ template <> struct Io<__half> {
   static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
 };
 
-// V consecutive values at element `at` of a row that is read once: 16-byte accesses that stay out of L1,
-// which keeps its room for the modulation rows.
-template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* p, int at, float (&x)[V]) {
-  if constexpr (V == 1) {
-    x[0] = Io<T>::get(p[at]);
-  } else {
-    constexpr int kWords = V * sizeof(T) / 16;
-    uint4 w[kWords];
+// Two 16-bit values in a word <-> fp32 (taken as words: 16-bit values one by one cost twice the instructions).
+template <typename T> struct Word;
+template <> struct Word<__nv_bfloat16> {
+  static __device__ __forceinline__ void get(uint32_t w, float& lo, float& hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t put(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+template <> struct Word<__half> {
+  static __device__ __forceinline__ void get(uint32_t w, float& lo, float& hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+  static __device__ __forceinline__ uint32_t put(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+
+// The arithmetic runs on packed pairs (V = 8) or on single values (V = 1).
+template <int V> struct Lane { using E = uint64_t; static constexpr int N = V / 2; };
+template <> struct Lane<1> { using E = float; static constexpr int N = 1; };
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mad(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float mad(float a, float b, float c) { return fmaf(a, b, c); }
+template <typename E> __device__ __forceinline__ E both(float x);
+template <> __device__ __forceinline__ uint64_t both<uint64_t>(float x) { return pair(x, x); }
+template <> __device__ __forceinline__ float both<float>(float x) { return x; }
+__device__ __forceinline__ float total(uint64_t x) {
+  float lo, hi;
+  split(x, lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ float total(float x) { return x; }
+
+// V consecutive values as they lie in memory: V = 8 in 16-byte words, V = 1 alone.
+template <typename T, int V> struct Raw {
+  static constexpr int kWords = V * sizeof(T) / 16;
+  uint4 w[kWords];
+  // of a row that is read once: past L1, which keeps its room for the modulation rows
+  __device__ __forceinline__ void load_once(const T* p) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i)
       asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "l"(reinterpret_cast<const uint4*>(p + at) + i));
-    const T* t = reinterpret_cast<const T*>(w);
+                   : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "l"(reinterpret_cast<const uint4*>(p) + i));
+  }
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = Io<T>::get(t[i]);
+    for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) *(reinterpret_cast<uint4*>(p) + i) = w[i];
+  }
+  __device__ __forceinline__ void get(uint64_t (&x)[V / 2]) const {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      float lo, hi;
+      if constexpr (sizeof(T) == 4) { lo = __uint_as_float(u[2 * i]); hi = __uint_as_float(u[2 * i + 1]); }
+      else Word<T>::get(u[i], lo, hi);
+      x[i] = pair(lo, hi);
+    }
+  }
+  __device__ __forceinline__ void put(const uint64_t (&x)[V / 2]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      float lo, hi;
+      split(x[i], lo, hi);
+      if constexpr (sizeof(T) == 4) { u[2 * i] = __float_as_uint(lo); u[2 * i + 1] = __float_as_uint(hi); }
+      else u[i] = Word<T>::put(lo, hi);
+    }
+  }
+};
+template <typename T> struct Raw<T, 1> {
+  T w;
+  __device__ __forceinline__ void load_once(const T* p) { w = *p; }
+  __device__ __forceinline__ void load(const T* p) { w = __ldg(p); }
+  __device__ __forceinline__ void store(T* p) const { *p = w; }
+  __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = Io<T>::get(w); }
+  __device__ __forceinline__ void put(const float (&x)[1]) { w = Io<T>::put(x[0]); }
+};
+
+enum { kAdd, kMul, kScale };
+// x (op) the modulation row `v`, which starts at element `at` for this thread: x + v, x v, x (1 + v).
+template <int OP, typename R, int V, int TPR, int VPT, typename E>
+__device__ __forceinline__ void apply_as(const void* ptr, int64_t at, int t, int nvec, E (&x)[VPT][Lane<V>::N]) {
+  const R* p = reinterpret_cast<const R*>(ptr) + at;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    if (t + TPR * k >= nvec) continue;
+    Raw<R, V> raw;
+    raw.load(p + TPR * k * V);
+    E v[Lane<V>::N];
+    raw.get(v);
+#pragma unroll
+    for (int i = 0; i < Lane<V>::N; ++i)
+      x[k][i] = OP == kAdd ? add(x[k][i], v[i]) : OP == kMul ? mul(x[k][i], v[i]) : mad(x[k][i], v[i], x[k][i]);
   }
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_row(T* p, int at, const float (&x)[V]) {
-  if constexpr (V == 1) {
-    p[at] = Io<T>::put(x[0]);
-  } else {
-    constexpr int kWords = V * sizeof(T) / 16;
-    uint4 w[kWords];
-    T* t = reinterpret_cast<T*>(w);
-#pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = Io<T>::put(x[i]);
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) *(reinterpret_cast<uint4*>(p + at) + i) = w[i];
-  }
-}
-template <typename T, int V>
-__device__ __forceinline__ void load_plain(const T* p, int at, float (&x)[V]) {
-  if constexpr (V == 1) {
-    x[0] = Io<T>::get(__ldg(p + at));
-  } else {
-    constexpr int kWords = V * sizeof(T) / 16;
-    uint4 w[kWords];
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p + at) + i);
-    const T* t = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = Io<T>::get(t[i]);
-  }
-}
-template <typename T, int V>
-__device__ __forceinline__ void load_vec(const RowVec& v, int64_t off, int at, float (&x)[V]) {
-  if (v.f32) load_plain<float, V>(reinterpret_cast<const float*>(v.ptr) + off, at, x);
-  else load_plain<T, V>(reinterpret_cast<const T*>(v.ptr) + off, at, x);
+template <int OP, typename T, int V, int TPR, int VPT, typename E>
+__device__ __forceinline__ void apply(const RowVec& v, int b, int row, int t, int nvec, E (&x)[VPT][Lane<V>::N]) {
+  if (!v.ptr) return;
+  const int64_t at = b * v.stride_b + row * v.stride_row + t * V;
+  if (v.f32) apply_as<OP, float, V, TPR, VPT>(v.ptr, at, t, nvec, x);
+  else apply_as<OP, T, V, TPR, VPT>(v.ptr, at, t, nvec, x);
 }
 
 // Sum over the TPR threads of a row.  The shared buffer alternates, so one barrier per sum is enough: a
@@ -119,136 +204,131 @@ __device__ __forceinline__ float row_sum(float x, float* red, int& turn) {
   return x;
 }
 
-// Mean (LayerNorm; 0 for RMSNorm) and reciprocal root of the mean square of a row held in registers.
-template <int V, int TPR, int VPT>
-__device__ __forceinline__ void row_stats(const NormArgs& a, int how, const float (&x)[VPT][V], int t, float* red,
-                                          int& turn, float& mean, float& rstd) {
-  mean = 0.f;
+// x <- (x - mean) / rms of a row held in registers (RMSNorm: the mean counts as 0).
+template <int V, int TPR, int VPT, typename E>
+__device__ __forceinline__ void normalise(const NormArgs& a, int how, E (&x)[VPT][Lane<V>::N], int t, float* red, int& turn) {
   if (how == XDIT_NORM_LAYER) {
-    float sum = 0.f;
+    E sum = both<E>(0.f);
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum += x[k][i];  // vectors behind the row are zero
-    mean = row_sum<TPR>(sum, red, turn) / (float)a.C;
+      for (int i = 0; i < Lane<V>::N; ++i) sum = add(sum, x[k][i]);  // vectors behind the row are zero
+    const E mean = both<E>(-row_sum<TPR>(total(sum), red, turn) / (float)a.C);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+#pragma unroll
+      for (int i = 0; i < Lane<V>::N; ++i) x[k][i] = add(x[k][i], mean);
   }
-  float sq = 0.f;
+  E sq = both<E>(0.f);
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
     if (t + TPR * k < a.nvec) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) sq = fmaf(x[k][i] - mean, x[k][i] - mean, sq);
+      for (int i = 0; i < Lane<V>::N; ++i) sq = mad(x[k][i], x[k][i], sq);
     }
-  rstd = rsqrtf(row_sum<TPR>(sq, red, turn) / (float)a.C + a.eps);
+  const E rstd = both<E>(rsqrtf(row_sum<TPR>(total(sq), red, turn) / (float)a.C + a.eps));
+#pragma unroll
+  for (int k = 0; k < VPT; ++k)
+#pragma unroll
+    for (int i = 0; i < Lane<V>::N; ++i) x[k][i] = mul(x[k][i], rstd);
 }
 
 template <int TPR> constexpr int kRowsPerCta = TPR == 32 ? 4 : 1;
 
+// A row's vectors are requested while the row before it is worked on.
 template <typename T, int V, int TPR, int VPT>
-__global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>)
+__global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>, TPR == 128 && VPT == 5 ? 4 : 1)
 gated_residual_norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[2 * (TPR / 32)];
-  constexpr int kRows = kRowsPerCta<TPR>;
+  using E = typename Lane<V>::E;
+  constexpr int N = Lane<V>::N, kRows = kRowsPerCta<TPR>;
   const int t = threadIdx.x % TPR;
+  const int step = gridDim.x * kRows;
   int turn = 0;
-  for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; r < a.rows; r += (int64_t)gridDim.x * kRows) {
-    const int b = (int)r / a.s, row = (int)r - b * a.s;
-    auto at_vec = [&](const RowVec& v) { return b * v.stride_b + row * v.stride_row; };
-    float h[VPT][V];
-    const T* res = reinterpret_cast<const T*>(a.residual) + b * a.r_sb + row * a.r_srow;
+  Raw<T, V> res[VPT], br[VPT];
+  auto fetch = [&](int r) {
+    const int b = r / a.s, row = r - b * a.s;
+    const T* p = reinterpret_cast<const T*>(a.residual) + b * a.r_sb + row * a.r_srow + t * V;
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int idx = t + TPR * k;
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = 0.f;
-      if (idx < a.nvec) load_row<T, V>(res, idx * V, h[k]);
-    }
+    for (int k = 0; k < VPT; ++k)
+      if (t + TPR * k < a.nvec) res[k].load_once(p + TPR * k * V);
     if (a.branch) {
-      float y[VPT][V];
-      const T* br = reinterpret_cast<const T*>(a.branch) + b * a.y_sb + row * a.y_srow;
-#pragma unroll
-      for (int k = 0; k < VPT; ++k) {
-        const int idx = t + TPR * k;
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[k][i] = 0.f;
-        if (idx < a.nvec) load_row<T, V>(br, idx * V, y[k]);
-      }
-      float mean = 0.f, rstd = 1.f;
-      if (a.post != XDIT_NORM_NONE) row_stats<V, TPR, VPT>(a, a.post, y, t, red, turn, mean, rstd);
-#pragma unroll
-      for (int k = 0; k < VPT; ++k) {
-        const int idx = t + TPR * k;
-        if (idx >= a.nvec) continue;
-        float v[V];
-        if (a.post != XDIT_NORM_NONE) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) y[k][i] = (y[k][i] - mean) * rstd;
-          if (a.post_weight.ptr) {
-            load_vec<T, V>(a.post_weight, 0, idx * V, v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[k][i] *= v[i];
-          }
-          if (a.post_bias.ptr) {
-            load_vec<T, V>(a.post_bias, 0, idx * V, v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[k][i] += v[i];
-          }
-        }
-        if (a.gate.ptr) {
-          load_vec<T, V>(a.gate, at_vec(a.gate), idx * V, v);
-#pragma unroll
-          for (int i = 0; i < V; ++i) y[k][i] *= v[i];
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[k][i] = fmaf(a.residual_scale, h[k][i], y[k][i]);
-      }
-    }
-    if (a.out_h) {
-      T* o = reinterpret_cast<T*>(a.out_h) + b * a.h_sb + row * a.h_srow;
+      const T* q = reinterpret_cast<const T*>(a.branch) + b * a.y_sb + row * a.y_srow + t * V;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (t + TPR * k < a.nvec) store_row<T, V>(o, (t + TPR * k) * V, h[k]);
+        if (t + TPR * k < a.nvec) br[k].load_once(q + TPR * k * V);
     }
-    if (a.norm == XDIT_NORM_NONE) continue;
-    float mean, rstd;
-    row_stats<V, TPR, VPT>(a, a.norm, h, t, red, turn, mean, rstd);
+  };
+  auto write = [&](void* out, int64_t at, const E (&x)[VPT][N]) {
+    T* o = reinterpret_cast<T*>(out) + at + t * V;
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int idx = t + TPR * k;
-      if (idx < a.nvec) {
-        float v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[k][i] = (h[k][i] - mean) * rstd;
-        if (a.weight.ptr) {
-          load_vec<T, V>(a.weight, 0, idx * V, v);
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[k][i] *= v[i];
-        }
-        if (a.bias.ptr) {
-          load_vec<T, V>(a.bias, 0, idx * V, v);
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[k][i] += v[i];
-        }
-        if (a.scale.ptr) {
-          load_vec<T, V>(a.scale, at_vec(a.scale), idx * V, v);
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[k][i] = fmaf(h[k][i], v[i], h[k][i]);
-        }
-        if (a.shift.ptr) {
-          load_vec<T, V>(a.shift, at_vec(a.shift), idx * V, v);
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[k][i] += v[i];
-        }
-        if (!a.out_q)
-          store_row<T, V>(reinterpret_cast<T*>(a.out_z) + b * a.z_sb + row * a.z_srow, idx * V, h[k]);
+    for (int k = 0; k < VPT; ++k)
+      if (t + TPR * k < a.nvec) {
+        Raw<T, V> w;
+        w.put(x[k]);
+        w.store(o + TPR * k * V);
       }
-      if constexpr (V == 8) {
-        if (a.out_q) {
+  };
+  int r = blockIdx.x * kRows + threadIdx.x / TPR;
+  if (r < a.rows) fetch(r);
+  for (; r < a.rows; r += step) {
+    const int b = r / a.s, row = r - b * a.s;
+    E h[VPT][N];
+    auto zero = [&](E (&x)[VPT][N]) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[k][i] = both<E>(0.f);
+    };
+    zero(h);
+    if (a.branch) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+        if (t + TPR * k < a.nvec) br[k].get(h[k]);
+      if (a.post != XDIT_NORM_NONE) {
+        normalise<V, TPR, VPT>(a, a.post, h, t, red, turn);
+        apply<kMul, T, V, TPR, VPT>(a.post_weight, b, row, t, a.nvec, h);
+        apply<kAdd, T, V, TPR, VPT>(a.post_bias, b, row, t, a.nvec, h);
+      }
+      apply<kMul, T, V, TPR, VPT>(a.gate, b, row, t, a.nvec, h);
+      const E rs = both<E>(a.residual_scale);
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        if (t + TPR * k >= a.nvec) {  // a normalised row has values behind its end
+#pragma unroll
+          for (int i = 0; i < N; ++i) h[k][i] = both<E>(0.f);
+          continue;
+        }
+        E x[N];
+        res[k].get(x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[k][i] = mad(rs, x[i], h[k][i]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+        if (t + TPR * k < a.nvec) res[k].get(h[k]);
+    }
+    if (r + step < a.rows) fetch(r + step);
+    if (a.out_h) write(a.out_h, b * a.h_sb + row * a.h_srow, h);
+    if (a.norm == XDIT_NORM_NONE) continue;
+    normalise<V, TPR, VPT>(a, a.norm, h, t, red, turn);
+    apply<kMul, T, V, TPR, VPT>(a.weight, b, row, t, a.nvec, h);
+    apply<kAdd, T, V, TPR, VPT>(a.bias, b, row, t, a.nvec, h);
+    apply<kScale, T, V, TPR, VPT>(a.scale, b, row, t, a.nvec, h);
+    apply<kAdd, T, V, TPR, VPT>(a.shift, b, row, t, a.nvec, h);
+    if constexpr (V == 8) {
+      if (a.out_q) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
           // 16 consecutive threads hold a block of 128; those behind the row add nothing to its maximum
-          float top = 0.f;
+          const int idx = t + TPR * k;
+          float x[8], top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) split(h[k][i], x[2 * i], x[2 * i + 1]);
           if (idx < a.nvec) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = amax_nan(top, h[k][i]);
+            for (int i = 0; i < 8; ++i) top = amax_nan(top, x[i]);
           }
 #pragma unroll
           for (int m = 8; m > 0; m >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
@@ -256,43 +336,59 @@ gated_residual_norm_kernel(const __grid_constant__ NormArgs a) {
           const float sc = block_scale(top, inv);
           if (idx < a.nvec) {
             uint2 q;
-            q.x = pack_e4m3(h[k][0] * inv, h[k][1] * inv, h[k][2] * inv, h[k][3] * inv);
-            q.y = pack_e4m3(h[k][4] * inv, h[k][5] * inv, h[k][6] * inv, h[k][7] * inv);
-            *reinterpret_cast<uint2*>(a.out_q + r * a.C + idx * 8) = q;
+            q.x = pack_e4m3(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            q.y = pack_e4m3(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+            *reinterpret_cast<uint2*>(a.out_q + (int64_t)r * a.C + idx * 8) = q;
             if (idx % 16 == 0) a.out_scale[(idx / 16) * a.scale_ld + r] = sc;
           }
         }
+        continue;
       }
     }
+    write(a.out_z, b * a.z_sb + row * a.z_srow, h);
   }
 }
 
-// Rows of a tensor to e4m3 with one scale for each block of 128: 16 threads per block of 128.
+// Rows of a tensor to e4m3 with one scale for each block of 128: a CTA walks whole rows, 16 threads hold a block, and
+// four vectors of a thread are on their way at a time.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kQuantThreads)
 quantize_rows_kernel(const T* x, int64_t sb, int64_t srow, int s, int64_t rows, int K, uint8_t* q, float* scale,
                      int64_t ld) {
-  const int kb = (K + kBlock - 1) / kBlock;
-  const int64_t items = rows * kb * 16;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < ((items + 31) / 32) * 32; i += (int64_t)gridDim.x * 256) {
-    const int64_t blk = i >> 4, r = blk / kb;
-    const int c = (int)(blk - r * kb), col = c * kBlock + (int)(i & 15) * 8;
-    const bool live = i < items && col < K;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) load_row<T, 8>(x + (r / s) * sb + (r % s) * srow, col, v);
-    float top = 0.f;
+  constexpr int kUnroll = 4;
+  const int nvec = K / 8, t = threadIdx.x;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* src = x + (r / s) * sb + (r % s) * srow;
+    for (int v0 = 0; v0 < nvec; v0 += kUnroll * kQuantThreads) {
+      Raw<T, 8> w[kUnroll];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = amax_nan(top, v[j]);
+      for (int u = 0; u < kUnroll; ++u)
+        if (v0 + u * kQuantThreads + t < nvec) w[u].load_once(src + (v0 + u * kQuantThreads + t) * 8);
 #pragma unroll
-    for (int m = 8; m > 0; m >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
-    float inv;
-    const float sc = block_scale(top, inv);
-    if (live) {
-      uint2 o;
-      o.x = pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-      o.y = pack_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-      *reinterpret_cast<uint2*>(q + r * K + col) = o;
-      if ((i & 15) == 0) scale[c * ld + r] = sc;
+      for (int u = 0; u < kUnroll; ++u) {
+        const int idx = v0 + u * kQuantThreads + t;
+        if (v0 + u * kQuantThreads >= nvec) break;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, top = 0.f;
+        if (idx < nvec) {
+          uint64_t p[4];
+          w[u].get(p);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) split(p[j], v[2 * j], v[2 * j + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = amax_nan(top, v[j]);
+#pragma unroll
+        for (int m = 8; m > 0; m >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
+        float inv;
+        const float sc = block_scale(top, inv);
+        if (idx < nvec) {
+          uint2 o;
+          o.x = pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+          o.y = pack_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+          *reinterpret_cast<uint2*>(q + r * K + idx * 8) = o;
+          if ((idx & 15) == 0) scale[(idx >> 4) * ld + r] = sc;
+        }
+      }
     }
   }
 }
@@ -312,7 +408,14 @@ quantize_weight_kernel(const T* w, int64_t srow, int N, int K, uint8_t* q, float
   for (int k = 0; k < 8; ++k) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
-    if (row0 + 16 * k < N && col < K) load_row<T, 8>(w + (row0 + 16 * k) * srow, col, v[k]);
+    if (row0 + 16 * k < N && col < K) {
+      Raw<T, 8> raw;
+      uint64_t p[4];
+      raw.load_once(w + (row0 + 16 * k) * srow + col);
+      raw.get(p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split(p[j], v[k][2 * j], v[k][2 * j + 1]);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = amax_nan(top, v[k][j]);
   }
@@ -336,16 +439,26 @@ quantize_weight_kernel(const T* w, int64_t srow, int N, int K, uint8_t* q, float
   if (threadIdx.x == 0) scale[blockIdx.x] = sc;
 }
 
+// CTAs of a kernel that an SM holds.
+template <typename F>
+int resident_ctas(F* kernel, int threads) {
+  int n = 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) == cudaSuccess && n > 0 ? n : 1;
+}
+
 template <typename T, int V, int TPR, int VPT>
 cudaError_t launch(const NormArgs& a, int sms, cudaStream_t stream) {
   constexpr int kRows = kRowsPerCta<TPR>, kThreads = TPR * kRows;
-  int64_t ctas = ((int64_t)a.rows + kRows - 1) / kRows, most = (int64_t)sms * (2048 / kThreads);
+  const int64_t ctas = ((int64_t)a.rows + kRows - 1) / kRows;
+  // as many CTAs as run at a time: each walks its rows with the next one's loads in flight
+  static const int resident = resident_ctas(gated_residual_norm_kernel<T, V, TPR, VPT>, kThreads);
+  const int64_t most = (int64_t)sms * resident;
   gated_residual_norm_kernel<T, V, TPR, VPT><<<(int)(ctas < most ? ctas : most), kThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 // Threads and vectors per thread of a row: as few threads as hold it in five vectors each (one warp up to
-// 1280 values: no barrier between a row's loads and its stores).
+// 1280 values: no barrier between a row's loads and its stores).  Rows that 16-byte words do not fit go value by value.
 template <typename T>
 cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
 #define XDIT_VPT5(V, TPR)                                       \
@@ -362,9 +475,10 @@ cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
     XDIT_VPT5(8, 512)
   }
 #undef XDIT_VPT5
-  if (a.nvec <= 1024) return launch<T, 1, 128, 8>(a, sms, stream);
+  if (a.nvec <= 512) return launch<T, 1, 128, 4>(a, sms, stream);
+  if (a.nvec <= 1280) return launch<T, 1, 128, 10>(a, sms, stream);
   if (a.nvec <= 4096) return launch<T, 1, 512, 8>(a, sms, stream);
-  return launch<T, 1, 512, 40>(a, sms, stream);
+  return launch<T, 1, 512, 32>(a, sms, stream);
 }
 
 bool aligned_rows(const void* p, int64_t sb, int64_t srow, int es, const xdit_norm_params& q) {
@@ -377,7 +491,7 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
   const char* who = "xdit_gated_residual_norm";
   const int es = dtype_size(p.dtype);
   if (!es) { set_error("%s: bad dtype %d", who, p.dtype); return XDIT_E_DTYPE; }
-  if (p.B < 0 || p.s < 0 || p.C < 1 || p.C > XDIT_NORM_MAX_C || (int64_t)p.B * p.s > 0x7fffffffll) {
+  if (p.B < 0 || p.s < 0 || p.C < 1 || p.C > XDIT_NORM_MAX_C || (int64_t)p.B * p.s > 0x7f000000ll) {
     set_error("%s: B=%d s=%d C=%d (C at most %d)", who, p.B, p.s, p.C, XDIT_NORM_MAX_C);
     return XDIT_E_SHAPE;
   }
@@ -463,18 +577,16 @@ int xdit_quantize_rows(const void* x, int64_t stride_b, int64_t stride_row, int3
     set_error("%s: rows must start on 16-byte boundaries", who);
     return XDIT_E_ALIGN;
   }
-  int sms = 0;
-  int rc = check_device(&sms);
+  int rc = check_device(nullptr);
   if (rc) return rc;
-  const int64_t blocks = (rows * ((K + kBlock - 1) / kBlock) * 16 + 255) / 256, most = (int64_t)sms * 32;
-  const int grid = (int)(blocks < most ? blocks : most);
+  const int grid = (int)(rows < 0x7fffffffll ? rows : 0x7fffffffll);
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == XDIT_BF16)
-    quantize_rows_kernel<<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, stride_b, stride_row, s, rows, K, (uint8_t*)q, scale, scale_ld);
+    quantize_rows_kernel<<<grid, kQuantThreads, 0, st>>>((const __nv_bfloat16*)x, stride_b, stride_row, s, rows, K, (uint8_t*)q, scale, scale_ld);
   else if (dtype == XDIT_F16)
-    quantize_rows_kernel<<<grid, 256, 0, st>>>((const __half*)x, stride_b, stride_row, s, rows, K, (uint8_t*)q, scale, scale_ld);
+    quantize_rows_kernel<<<grid, kQuantThreads, 0, st>>>((const __half*)x, stride_b, stride_row, s, rows, K, (uint8_t*)q, scale, scale_ld);
   else
-    quantize_rows_kernel<<<grid, 256, 0, st>>>((const float*)x, stride_b, stride_row, s, rows, K, (uint8_t*)q, scale, scale_ld);
+    quantize_rows_kernel<<<grid, kQuantThreads, 0, st>>>((const float*)x, stride_b, stride_row, s, rows, K, (uint8_t*)q, scale, scale_ld);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "quantize_rows_kernel launch");
   return XDIT_OK;

@@ -8,9 +8,10 @@
 // product is taken in 64 bits and counted in turns (f / 2 pi), the whole turns are dropped, and only the
 // fraction goes to 32 bits for sincospi.
 //
-// HBM-bound: q and k are read and written once.  A thread owns one vector of one token's head (its
-// column does not change from head to head) and walks the heads of q and k, so the angles are computed
-// once per thread and stay in registers.
+// HBM-bound: q and k are read and written once.  A CTA takes a few tokens and many heads of q and k: it computes the
+// tokens' angles once, into shared memory, while its first vectors are on their way, and then walks its vectors in
+// the order in which they lie in memory (heads of a token, or tokens of a head, whichever are nearer), so that
+// loads and stores cover runs of 4 KB.
 #include <cstring>
 
 #include "common.cuh"
@@ -19,7 +20,7 @@ namespace xdit {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // heads whose vectors a thread has in flight
+constexpr int kMaxTokens = 16; // tokens of a CTA
 
 struct RotaryArgs {
   const char* src[2];
@@ -27,38 +28,44 @@ struct RotaryArgs {
   int64_t ss_b[2], ss_h[2], ss_row[2];  // elements
   int64_t ds_b[2], ds_h[2], ds_row[2];
   int32_t heads[2];
-  int64_t rows;      // B * s
   int32_t s, D, rot;
-  int32_t slots;     // vectors of a head that threads own
-  int32_t splits, per_split;  // heads (of q and k together) are split over `splits` threads
+  int32_t slots;       // vectors of a head (pairs of vectors where a rotation takes two)
+  int32_t tokens;      // tokens of a CTA, all of one sample
+  int32_t blocks_s;    // CTAs along the tokens of a sample
+  int32_t per_split;   // heads of a CTA, all of q or all of k
+  int32_t splits_q;    // CTAs along the heads of q; those of k follow
+  int32_t heads_first; // a token's heads lie nearer to each other than a head's tokens
   // positions
   const void* pos;
   int64_t pos_sb, pos_srow, pos_saxis;
   int32_t pos_kind, axes;
   int64_t grid[XDIT_ROTARY_MAX_AXES], start;
+  int32_t grid_small;  // the grid's tokens can be counted in 32 bits
   double turns[XDIT_ROTARY_MAX_PAIRS];  // frequency / 2 pi
   uint8_t axis[XDIT_ROTARY_MAX_PAIRS];
 };
 
+template <typename I>
+__device__ __forceinline__ double grid_position(const RotaryArgs& a, I n, int axis) {
+  // the last axis runs fastest; tokens behind the grid (padding of a shard) stay at the origin
+  I below = 1, volume = 1;
+  for (int i = 0; i < a.axes; ++i) {
+    volume *= (I)a.grid[i];
+    if (i > axis) below *= (I)a.grid[i];
+  }
+  return n < volume ? (double)(n / below % (I)a.grid[axis]) : 0.0;
+}
 // Position of token (b, row) along `axis`.
 __device__ __forceinline__ double position(const RotaryArgs& a, int b, int row, int axis) {
-  if (a.pos_kind == XDIT_POS_GRID) {
-    // the last axis runs fastest; tokens behind the grid (padding of a shard) stay at the origin
-    int64_t n = a.start + row, below = 1, volume = 1;
-    for (int i = 0; i < a.axes; ++i) {
-      volume *= a.grid[i];
-      if (i > axis) below *= a.grid[i];
-    }
-    return n < volume ? (double)(n / below % a.grid[axis]) : 0.0;
-  }
+  if (a.pos_kind == XDIT_POS_GRID)
+    return a.grid_small ? grid_position<uint32_t>(a, (uint32_t)(a.start + row), axis) : grid_position<uint64_t>(a, (uint64_t)(a.start + row), axis);
   const int64_t at = b * a.pos_sb + row * a.pos_srow + axis * a.pos_saxis;
   if (a.pos_kind == XDIT_POS_I32) return (double)__ldg(reinterpret_cast<const int32_t*>(a.pos) + at);
   if (a.pos_kind == XDIT_POS_I64) return (double)__ldg(reinterpret_cast<const long long*>(a.pos) + at);
   return (double)__ldg(reinterpret_cast<const float*>(a.pos) + at);
 }
-
-__device__ __forceinline__ void turn(const RotaryArgs& a, int b, int row, int pair, float& c, float& s) {
-  const double t = position(a, b, row, a.axis[pair]) * a.turns[pair];
+__device__ __forceinline__ void turn(double position, double turns, float& c, float& s) {
+  const double t = position * turns;
   sincospif((float)(2.0 * (t - rint(t))), &s, &c);
 }
 
@@ -75,67 +82,146 @@ template <> struct Io<__half> {
   static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
 };
-template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T x[V]; };
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec { T x[V]; };
+// What a slot's access moves: whole words, so that the compiler does not take 16-bit values apart.
+template <int BYTES> struct RawOf { using type = Vec<uint32_t, BYTES / 4>; };
+template <> struct RawOf<2> { using type = Vec<uint16_t, 1>; };
 
-// A slot is what one thread owns of a head.  Interleaved pairs: one vector of V elements (V/2 pairs; for
-// V = 1 one pair in two scalar accesses).  Halves: the vectors at i and i + rot/2.  Slots behind the
-// rotated part hold one vector that is copied.
-template <typename T, int V, bool HALVES>
-__global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr bool kTwo = HALVES || V == 1;        // two accesses per rotating slot
-  constexpr int kPairs = kTwo ? V : V / 2;       // pairs per rotating slot
-  using Vt = Vec<T, V>;
-  const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t token = item / a.slots;
-  if (token >= a.rows * a.splits) return;
-  const int slot = (int)(item - token * a.slots);
-  const int64_t r = token / a.splits;
-  const int split = (int)(token - r * a.splits);
-  const int b = (int)(r / a.s), row = (int)(r - (int64_t)b * a.s);
-  const int rotating = a.rot / 2 / kPairs;
-  const bool rotates = slot < rotating;
-  int at0, at1 = 0;
-  if (!rotates) at0 = a.rot + (slot - rotating) * V;
-  else if (HALVES) { at0 = slot * V; at1 = at0 + a.rot / 2; }
-  else if (V == 1) { at0 = 2 * slot; at1 = at0 + 1; }
-  else at0 = slot * V;
-  float c[kPairs], s[kPairs];
-#pragma unroll
-  for (int p = 0; p < kPairs; ++p) { c[p] = 1.f; s[p] = 0.f; }
-  if (rotates) {
-#pragma unroll
-    for (int p = 0; p < kPairs; ++p) turn(a, b, row, slot * kPairs + p, c[p], s[p]);
+// Two 16-bit values in a word <-> fp32.
+template <typename T> struct Word;
+template <> struct Word<__nv_bfloat16> {
+  static __device__ __forceinline__ void get(uint32_t w, float& lo, float& hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
   }
-  const int first = split * a.per_split, last = min(first + a.per_split, a.heads[0] + a.heads[1]);
-  for (int h0 = first; h0 < last; h0 += kUnroll) {
-    Vt x[kUnroll], y[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int g = h0 + u;
-      if (g >= last) break;
-      const int t = g >= a.heads[0], h = t ? g - a.heads[0] : g;
-      const T* src = reinterpret_cast<const T*>(a.src[t]) + b * a.ss_b[t] + h * a.ss_h[t] + row * a.ss_row[t];
-      x[u] = *reinterpret_cast<const Vt*>(src + at0);
-      if (kTwo && rotates) y[u] = *reinterpret_cast<const Vt*>(src + at1);
+  static __device__ __forceinline__ uint32_t put(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+template <> struct Word<__half> {
+  static __device__ __forceinline__ void get(uint32_t w, float& lo, float& hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+  static __device__ __forceinline__ uint32_t put(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+__device__ __forceinline__ void rotate(float& x, float& y, float c, float s) {
+  const float z = x;
+  x = x * c - y * s;
+  y = z * s + y * c;
+}
+
+// A slot is one thread's part of a head.  Interleaved pairs: one vector of V elements (V/2 pairs; for
+// V = 1 one pair in two scalar accesses).  Halves: the vectors at i and i + rot/2.  Slots behind the
+// rotated part hold one vector that is copied.  A thread keeps its slot and steps over (token, head) with
+// constant strides: what is left per vector is the rotation itself.
+template <typename T, int V, bool HALVES>
+__global__ void __launch_bounds__(kThreads, HALVES ? 5 : 7) rotary_axes_kernel(const __grid_constant__ RotaryArgs a) {
+  extern __shared__ __align__(16) float angles[];  // cos [tokens][pairs], sin [tokens][pairs]
+  __shared__ double places[kMaxTokens * XDIT_ROTARY_MAX_AXES], turns[XDIT_ROTARY_MAX_PAIRS];
+  __shared__ uint8_t axis[XDIT_ROTARY_MAX_PAIRS];
+  constexpr bool kTwo = HALVES || V == 1;   // two accesses per rotating slot
+  constexpr int kPairs = kTwo ? V : V / 2;  // pairs per rotating slot
+  using Vt = typename RawOf<sizeof(T) * V>::type;
+  using Ct = Vec<float, kPairs>;
+  const int b = blockIdx.x / a.blocks_s, row0 = (blockIdx.x - b * a.blocks_s) * a.tokens;
+  const int t = (int)blockIdx.y >= a.splits_q, head0 = ((int)blockIdx.y - (t ? a.splits_q : 0)) * a.per_split;
+  const int tokens = min(a.tokens, a.s - row0), heads = min(a.per_split, a.heads[t] - head0);
+  const int pairs = a.rot / 2, rotating = pairs / kPairs;
+  float* cosines = angles;
+  float* sines = angles + a.tokens * pairs;
+  const T* src = reinterpret_cast<const T*>(a.src[t]) + b * a.ss_b[t] + head0 * a.ss_h[t] + row0 * a.ss_row[t];
+  T* dst = reinterpret_cast<T*>(a.dst[t]) + b * a.ds_b[t] + head0 * a.ds_h[t] + row0 * a.ds_row[t];
+  // (outer, inner) = (token, head) or (head, token), whichever is the order in memory
+  const int n_in = a.heads_first ? heads : tokens, n_out = a.heads_first ? tokens : heads;
+  // offsets inside a CTA's part fit 32 bits: the launch sees to it
+  const int s_in = (int)(a.heads_first ? a.ss_h[t] : a.ss_row[t]), s_out = (int)(a.heads_first ? a.ss_row[t] : a.ss_h[t]);
+  const int d_in = (int)(a.heads_first ? a.ds_h[t] : a.ds_row[t]), d_out = (int)(a.heads_first ? a.ds_row[t] : a.ds_h[t]);
+  const int width = min(a.slots, kThreads), rows = kThreads / width;  // threads along a head, heads side by side
+  const int step_in = rows % n_in, step_out = rows / n_in;
+  const int s_step = step_in * s_in + step_out * s_out, s_wrap = s_out - n_in * s_in;
+  const int d_step = step_in * d_in + step_out * d_out, d_wrap = d_out - n_in * d_in;
+  const int y0 = threadIdx.x / width, total = n_in * n_out;
+  bool ready = false;
+  for (int slot0 = 0; slot0 < a.slots; slot0 += width) {
+    const int slot = slot0 + (int)threadIdx.x - y0 * width;
+    const bool rotates = slot < rotating;
+    int at0 = slot * V, at1 = 0;
+    if (!rotates) at0 = a.rot + (slot - rotating) * V;
+    else if (HALVES) at1 = at0 + pairs;
+    else if (V == 1) { at0 = 2 * slot; at1 = at0 + 1; }
+    const int apart = at1 - at0;
+    int in = y0 % n_in, out = y0 / n_in, y = slot < a.slots && y0 < rows ? y0 : total;
+    int so = in * s_in + out * s_out + at0, to = in * d_in + out * d_out + at0;
+    Vt x, w;
+    auto load = [&]() {
+      if (y >= total) return;
+      x = *reinterpret_cast<const Vt*>(src + so);
+      if (kTwo && rotates) w = *reinterpret_cast<const Vt*>(src + so + apart);
+    };
+    load();
+    if (!ready) {  // while the first vectors are on their way
+      for (int i = threadIdx.x; i < tokens * a.axes; i += kThreads)
+        places[i] = position(a, b, row0 + i / a.axes, i % a.axes);
+      for (int i = threadIdx.x; i < pairs; i += kThreads) {  // an argument read at a place of each lane's own is slow
+        turns[i] = a.turns[i];
+        axis[i] = a.axis[i];
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
+        const int n = i / pairs, pair = i - n * pairs;
+        turn(places[n * a.axes + axis[pair]], turns[pair], cosines[i], sines[i]);
+      }
+      __syncthreads();
+      ready = true;
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int g = h0 + u;
-      if (g >= last) break;
-      const int t = g >= a.heads[0], h = t ? g - a.heads[0] : g;
-      T* dst = reinterpret_cast<T*>(a.dst[t]) + b * a.ds_b[t] + h * a.ds_h[t] + row * a.ds_row[t];
+    while (y < total) {
+      Vt o = x, o2 = w;
+      const int angle = (a.heads_first ? out : in) * pairs + slot * kPairs;
+      T* d = dst + to;
+      y += rows;
+      in += step_in; out += step_out; so += s_step; to += d_step;
+      if (in >= n_in) { in -= n_in; ++out; so += s_wrap; to += d_wrap; }
+      load();  // the next vector, while this one turns
       if (rotates) {
+        const Ct c = *reinterpret_cast<const Ct*>(cosines + angle);
+        const Ct s = *reinterpret_cast<const Ct*>(sines + angle);
+        if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-        for (int p = 0; p < kPairs; ++p) {
-          T& ta = kTwo ? x[u].x[p] : x[u].x[2 * p];
-          T& tb = kTwo ? y[u].x[p] : x[u].x[(2 * p + 1) % V];
-          const float va = Io<T>::get(ta), vb = Io<T>::get(tb);
-          ta = Io<T>::put(va * c[p] - vb * s[p]);
-          tb = Io<T>::put(va * s[p] + vb * c[p]);
+          for (int i = 0; i < V / 2; ++i) {
+            float x0, x1, y0, y1;
+            Word<T>::get(o.x[i], x0, x1);
+            if constexpr (HALVES) {
+              Word<T>::get(o2.x[i], y0, y1);
+              rotate(x0, y0, c.x[2 * i], s.x[2 * i]);
+              rotate(x1, y1, c.x[2 * i + 1], s.x[2 * i + 1]);
+              o2.x[i] = Word<T>::put(y0, y1);
+            } else {
+              rotate(x0, x1, c.x[i], s.x[i]);
+            }
+            o.x[i] = Word<T>::put(x0, x1);
+          }
+        } else {  // fp32, or one 16-bit value in an access
+          T* ta = reinterpret_cast<T*>(&o);
+          T* tb = reinterpret_cast<T*>(&o2);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            T& va = kTwo ? ta[i] : ta[2 * i];
+            T& vb = kTwo ? tb[i] : ta[(2 * i + 1) % V];
+            float x0 = Io<T>::get(va), x1 = Io<T>::get(vb);
+            rotate(x0, x1, c.x[i], s.x[i]);
+            va = Io<T>::put(x0);
+            vb = Io<T>::put(x1);
+          }
         }
       }
-      *reinterpret_cast<Vt*>(dst + at0) = x[u];
-      if (kTwo && rotates) *reinterpret_cast<Vt*>(dst + at1) = y[u];
+      *reinterpret_cast<Vt*>(d) = o;
+      if (kTwo && rotates) *reinterpret_cast<Vt*>(d + apart) = o2;
     }
   }
 }
@@ -149,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) rotary_tables_kernel(const __grid_co
   if (row >= a.s) return;
   const int pair = (int)(item - row * (a.D / 2));
   float c = 1.f, s = 0.f;
-  if (2 * pair < a.rot) turn(a, 0, (int)row, pair, c, s);
+  if (2 * pair < a.rot) turn(position(a, 0, (int)row, a.axis[pair]), a.turns[pair], c, s);
   *reinterpret_cast<float2*>(cos + row * a.D + 2 * pair) = make_float2(c, c);
   *reinterpret_cast<float2*>(sin + row * a.D + 2 * pair) = make_float2(s, s);
 }
@@ -177,6 +263,7 @@ int fill_positions(RotaryArgs& a, const xdit_rotary_positions& p, const char* wh
     }
     if (p.start < 0 || p.start > (1ll << 40)) { set_error("%s: start %lld", who, (long long)p.start); return XDIT_E_SHAPE; }
     a.start = p.start;
+    a.grid_small = volume < (1ll << 31) && p.start < (1ll << 31);  // start + row stays below 2^32
   } else {
     if (!p.positions) { set_error("%s: NULL positions", who); return XDIT_E_NULL; }
     a.pos = p.positions;
@@ -188,9 +275,10 @@ int fill_positions(RotaryArgs& a, const xdit_rotary_positions& p, const char* wh
 }
 
 template <typename T, int V>
-cudaError_t launch(const RotaryArgs& a, bool halves, int64_t blocks, cudaStream_t stream) {
-  if (halves) rotary_axes_kernel<T, V, true><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
-  else rotary_axes_kernel<T, V, false><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
+cudaError_t launch(const RotaryArgs& a, bool halves, dim3 grid, cudaStream_t stream) {
+  const size_t smem = (size_t)a.tokens * a.rot * sizeof(float);
+  if (halves) rotary_axes_kernel<T, V, true><<<grid, kThreads, smem, stream>>>(a);
+  else rotary_axes_kernel<T, V, false><<<grid, kThreads, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -215,7 +303,6 @@ int launch_rotary(const xdit_rotary_params& p, cudaStream_t stream) {
   a.src[0] = (const char*)p.q; a.src[1] = (const char*)p.k;
   a.dst[0] = (char*)p.out_q; a.dst[1] = (char*)p.out_k;
   a.heads[0] = p.H; a.heads[1] = p.Hk;
-  a.rows = (int64_t)p.B * p.s;
   a.s = p.s; a.D = p.D;
   // The widest vector that all addresses, strides and the split of a head into pairs allow.
   uint64_t low = 0;  // low bits of everything a vector access starts from, in bytes
@@ -231,26 +318,47 @@ int launch_rotary(const xdit_rotary_params& p, cudaStream_t stream) {
   int V = 16 / es;
   const int whole = halves ? a.rot / 2 : a.rot;
   while (V > 1 && ((low % (V * es)) || whole % V || (p.D - a.rot) % V)) V /= 2;
-  const int per = (halves || V == 1) ? V : V / 2;  // pairs of a rotating slot
-  a.slots = a.rot / 2 / per + (p.D - a.rot) / V;
-  // Threads walk all heads unless there are too few tokens to fill the GPU: then the heads are split until
-  // about 2048 threads per SM are at work (the angles are then computed once per split).
-  const int heads = p.H + p.Hk;
-  const int64_t items = a.rows * a.slots;
-  int64_t splits = ((int64_t)sms * 2048 + items - 1) / items;
-  if (splits > heads) splits = heads;
-  a.per_split = (int)((heads + splits - 1) / splits);
-  a.splits = (heads + a.per_split - 1) / a.per_split;
-  const int64_t blocks = (items * a.splits + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffll) { set_error("xdit_rotary_axes: too many tokens"); return XDIT_E_SHAPE; }
+  const int per_slot = (halves || V == 1) ? V : V / 2;  // pairs of a rotating slot
+  a.slots = a.rot / 2 / per_slot + (p.D - a.rot) / V;
+  // A CTA takes 16 tokens and all heads of q or of k; fewer tokens, and then fewer heads, while there are not two CTAs
+  // for every SM.
+  a.heads_first = p.H > 1 && a.ss_h[0] < a.ss_row[0];
+  a.tokens = kMaxTokens;
+  auto ctas = [&](int per) {
+    return (int64_t)p.B * ((p.s + a.tokens - 1) / a.tokens) * ((p.H + per - 1) / per + (p.Hk + per - 1) / per);
+  };
+  int per = p.H > p.Hk ? p.H : p.Hk;
+  while (a.tokens > 1 && ctas(per) < 2 * sms) a.tokens /= 2;
+  while (per > 1 && ctas(per) < 2 * sms && a.tokens * (int64_t)per * a.slots > kThreads) per = (per + 1) / 2;
+  // a CTA counts its offsets in 32 bits
+  auto reach = [&]() {
+    int64_t far = 0;
+    for (int t = 0; t < 2; ++t) {
+      const int64_t in = a.tokens * a.ss_row[t] + per * a.ss_h[t], out = a.tokens * a.ds_row[t] + per * a.ds_h[t];
+      far = in > far ? in : far;
+      far = out > far ? out : far;
+    }
+    return far + p.D;
+  };
+  while (a.tokens > 1 && reach() > 0x3fffffffll) a.tokens /= 2;
+  while (per > 1 && reach() > 0x3fffffffll) per = (per + 1) / 2;
+  a.blocks_s = (p.s + a.tokens - 1) / a.tokens;
+  a.per_split = per;
+  a.splits_q = (p.H + per - 1) / per;
+  const int splits = a.splits_q + (p.Hk + per - 1) / per;
+  if ((int64_t)p.B * a.blocks_s > 0x7fffffffll || splits > 65535 || (int64_t)a.tokens * per > 0x3fffffffll) {
+    set_error("xdit_rotary_axes: too many tokens or heads");
+    return XDIT_E_SHAPE;
+  }
+  const dim3 blocks_grid((unsigned)(p.B * a.blocks_s), splits);
   cudaError_t e;
 #define XDIT_LAUNCH_ROTARY(T)                                          \
-  (V == 8 ? launch<T, 8>(a, halves, blocks, stream) : V == 4 ? launch<T, 4>(a, halves, blocks, stream) \
-   : V == 2 ? launch<T, 2>(a, halves, blocks, stream) : launch<T, 1>(a, halves, blocks, stream))
+  (V == 8 ? launch<T, 8>(a, halves, blocks_grid, stream) : V == 4 ? launch<T, 4>(a, halves, blocks_grid, stream) \
+   : V == 2 ? launch<T, 2>(a, halves, blocks_grid, stream) : launch<T, 1>(a, halves, blocks_grid, stream))
   if (p.dtype == XDIT_BF16) e = XDIT_LAUNCH_ROTARY(__nv_bfloat16);
   else if (p.dtype == XDIT_F16) e = XDIT_LAUNCH_ROTARY(__half);
-  else e = V == 4 ? launch<float, 4>(a, halves, blocks, stream) : V == 2 ? launch<float, 2>(a, halves, blocks, stream)
-                                                              : launch<float, 1>(a, halves, blocks, stream);
+  else e = V == 4 ? launch<float, 4>(a, halves, blocks_grid, stream) : V == 2 ? launch<float, 2>(a, halves, blocks_grid, stream)
+                                                              : launch<float, 1>(a, halves, blocks_grid, stream);
 #undef XDIT_LAUNCH_ROTARY
   if (e != cudaSuccess) return cuda_fail(e, "rotary_axes_kernel launch");
   return XDIT_OK;
