@@ -438,6 +438,12 @@ struct xdit_fp8_linear_params {
   int64_t out_scale_ld;
   int32_t *status, *status_host;
   uint32_t wait_limit_ns;
+  /* Optional: x as it is before quantisation, [M / raw_s, raw_s, K] in raw_dtype (raw_s 0: one sample of M rows).
+   * It is quantised by the rule of xdit_quantize_rows into x and x_scale, which are then buffers of the caller:
+   * contiguous rows, x_scale_stride_row 1. */
+  int32_t raw_dtype, raw_s;
+  const void* raw;
+  int64_t raw_stride_b, raw_stride_row;
 };
 XDIT_API int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* stream);
 

@@ -62,4 +62,9 @@ int64_t attn_sm100_split_scratch_bytes(const xdit_attn_params& p);
 // ---- attention prologue (prologue.cu) ------------------------------------------------------------
 int launch_prologue(const xdit_prologue_params& p, cudaStream_t stream);
 
+// ---- e4m3 rows (modnorm.cu) ------------------------------------------------------------------------
+// Body of xdit_quantize_rows; `who` names the entry point in the reasons of a refusal.
+int launch_quantize_rows(const char* who, const void* x, int64_t stride_b, int64_t stride_row, int32_t dtype, int32_t B,
+                         int32_t s, int32_t K, void* q, float* scale, int64_t scale_ld, void* stream);
+
 }  // namespace xdit

@@ -53,6 +53,7 @@ struct alignas(64) GemmArgs {
   CUtensorMap tm_x, tm_w, tm_out;
   int32_t M, N, kb;        // kb: blocks along K
   int32_t mt, nt;          // tiles
+  int32_t splits;          // CTAs of a cluster that share the K axis of a tile (few rows)
   const float* xs;
   int64_t xs_srow, xs_skb;
   const float* ws;
@@ -76,6 +77,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
+// 32 lanes x 16 consecutive columns -> 16 registers per thread
+#define XDIT_TMEM_LD16(a, taddr)                                                                                   \
+  asm volatile(                                                                                                    \
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "                                                                     \
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"                              \
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),   \
+        "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])                    \
+      : "r"(taddr) : "memory")
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tm), "r"(src), "r"(c0), "r"(c1) : "memory");
 }
@@ -115,6 +124,16 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x
 __device__ __forceinline__ float gelu_tanh(float x) {
   const float u = 0.7978845608028654f * fmaf(0.044715f * x * x, x, x);
   return __fdividef(x, 1.f + __expf(-2.f * u));
+}
+// A CTA whose wait gave up tells the later launches and the host.
+__device__ __forceinline__ void report(const GemmArgs& a, volatile int* abort_flag) {
+  if (threadIdx.x == 0 && *abort_flag > 0) {
+    if (a.status) atomicCAS(a.status, 0, *abort_flag);
+    if (a.status_host) {  // host-visible copy, read by the next call without a synchronise
+      *reinterpret_cast<volatile int32_t*>(a.status_host) = *abort_flag;
+      __threadfence_system();
+    }
+  }
 }
 __device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& m, int& n) {
   const int band = t / (kBand * a.nt), rem = t - band * kBand * a.nt;
@@ -398,13 +417,295 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
   }
-  if (threadIdx.x == 0 && *abort_flag > 0) {
-    if (a.status) atomicCAS(a.status, 0, *abort_flag);
-    if (a.status_host) {  // host-visible copy, read by the next call without a synchronise
-      *reinterpret_cast<volatile int32_t*>(a.status_host) = *abort_flag;
-      __threadfence_system();
+  report(a, abort_flag);
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Few rows of x: the weight's bytes bound the time, so the operands change places.  A tile is 128 rows of W (the
+// M side of the MMA) by NB rows of x, small enough for two CTAs on an SM, with a deep ring of W in flight; a thread
+// holds NB sums of its row of W.  When there are fewer tiles than SMs can use, the K axis is split over the CTAs of a
+// cluster: each leaves its sums in shared memory, and each then adds the cluster's sums, in their order, for a share of the
+// rows of x -- no scratch in global memory, and the same result every time.
+//   warps 0-3  scaled sums + epilogue      warp 4  MMA      warp 5  TMA      warp 6  scales
+// The kernel may start while the one that quantises x is still running (griddepcontrol): W is loaded at once, x and
+// its scales after that kernel's end.
+constexpr int kRowsThreads = 224;
+
+template <int NB> struct RowsLayout {
+  static constexpr int kStages = NB <= 16 ? 6 : NB <= 32 ? 5 : 4;
+  static constexpr int kStageBytes = kABytes + NB * kBK;
+  static constexpr int kSlot = NB * 4 + 16;                   // scales of a step: NB of x, one of W
+  static constexpr int kAhead = 8, kGroup = 4, kGroups = kAhead / kGroup;
+  static constexpr int kScaleOff = kStages * kStageBytes;
+  static constexpr int kTopOff = kScaleOff + kAhead * kSlot;  // [4 warps][NB] largest magnitudes
+  static constexpr int kBarOff = kTopOff + 4 * NB * 4;
+  static constexpr int kNumBars = 2 * kStages + 4 + 1 + 2 * kGroups;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kSmem = kMiscOff + 16 + 1024;
+  static_assert(kStages * kStageBytes >= 128 * NB * 4, "the ring holds the sums that a cluster exchanges");
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 load_cluster(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_constant__ GemmArgs a) {
+  using L = RowsLayout<NB>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ unsigned char smem_dyn[];
+  const uint32_t raw = smem_u32(smem_dyn), base = (raw + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_dyn + (base - raw);
+  const uint32_t bar0 = base + L::kBarOff;
+  auto bar_full = [&](int s) { return bar0 + 8u * s; };
+  auto bar_empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto bar_tfull = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
+  auto bar_tempty = [&](int s) { return bar0 + 8u * (2 * kStages + 2 + s); };
+  const uint32_t bar_drain = bar0 + 8u * (2 * kStages + 4);
+  auto bar_sfull = [&](int s) { return bar0 + 8u * (2 * kStages + 5 + s); };
+  auto bar_sempty = [&](int s) { return bar0 + 8u * (2 * kStages + 5 + L::kGroups + s); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + L::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + L::kMiscOff + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kTmem = 2 * NB < 32 ? 32 : 2 * NB;
+  // blockIdx.x = (tile of W) * splits + split, blockIdx.y = tile of x
+  const int split = blockIdx.x % a.splits, n0 = (blockIdx.x / a.splits) * 128, m0 = blockIdx.y * NB;
+  const int c0 = (int)((int64_t)split * a.kb / a.splits), steps = (int)((int64_t)(split + 1) * a.kb / a.splits) - c0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(bar_tfull(s), 1); mbar_init(bar_tempty(s), 4); }
+    for (int s = 0; s < L::kGroups; ++s) { mbar_init(bar_sfull(s), 32); mbar_init(bar_sempty(s), 4); }
+    mbar_init(bar_drain, 1);
+    *abort_flag = status_is_set(a.status) ? -1 : 0;  // -1: skip all work (an earlier failure is pending)
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmem) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool skip = *abort_flag != 0;  // same value for every thread: written before the barrier above
+  bool ok = !skip;
+  float acc[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[i] = 0.f;
+
+  if (skip) {
+    // nothing to do: fall through to the teardown, which frees TMEM
+  } else if (warp == 5) {
+    // ======================= TMA producer =======================
+    if (lane == 0) {
+      auto load_w = [&](int i) {
+        mbar_arrive_expect_tx(bar_full(i % kStages), L::kStageBytes);
+        tma_load_2d(base + (i % kStages) * L::kStageBytes, &a.tm_w, bar_full(i % kStages), (c0 + i) * kBK, n0);
+      };
+      auto load_x = [&](int i) {
+        tma_load_2d(base + (i % kStages) * L::kStageBytes + kABytes, &a.tm_x, bar_full(i % kStages), (c0 + i) * kBK, m0);
+      };
+      const int first = min(steps, kStages);
+      for (int i = 0; i < first; ++i) load_w(i);
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // x is complete from here on
+      for (int i = 0; i < first; ++i) load_x(i);
+      int issued = first;
+      for (; issued < steps; ++issued) {
+        ok = mbar_wait(bar_empty(issued % kStages), (issued / kStages - 1) & 1, abort_flag, a.wait_limit_ns, 100);
+        if (!ok) break;
+        load_w(issued);
+        load_x(issued);
+      }
+      if (!ok) {
+        // drain: every armed stage must have received its bytes before the CTA may leave
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_full(i % kStages), (i / kStages) & 1); ++it) __nanosleep(64);
+      }
+    }
+  } else if (warp == 6) {
+    // ======================= scales =======================
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int kPer = (NB + 31) / 32;
+    const float* src[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int row = m0 + 32 * i + lane;  // rows behind the end take any scale
+      src[i] = a.xs + (int64_t)(row < a.M ? row : 0) * a.xs_srow + c0 * a.xs_skb;
+    }
+    const float* w = a.ws + (n0 / kBK) * a.ws_snb + c0 * a.ws_skb;
+    int step = 0;
+    for (; step < steps; ++step) {
+      const int slot = step % L::kAhead, turn = step / L::kAhead;
+      if (turn > 0 && step % L::kGroup == 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty(slot / L::kGroup), (turn - 1) & 1, abort_flag, a.wait_limit_ns, 320));
+      if (!ok) break;
+      const uint32_t at = base + L::kScaleOff + slot * L::kSlot;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (32 * i + lane < NB)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + (32 * i + lane) * 4), "l"(src[i]) : "memory");
+        src[i] += a.xs_skb;
+      }
+      if (lane == 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + NB * 4), "l"(w) : "memory");
+      w += a.ws_skb;
+      if (step % L::kGroup == L::kGroup - 1 || step == steps - 1)
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_sfull(slot / L::kGroup)) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 4) {
+    // ======================= MMA issuer (the warp runs converged, one elected lane issues) =======================
+    const bool leader = elect_one();
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+    const uint32_t idesc = (1u << 4) | ((uint32_t)(NB >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);  // e4m3 x e4m3 -> fp32
+    auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.wait_limit_ns, code));
+    };
+    for (int step = 0; step < steps; ++step) {
+      const int st = step % kStages, buf = step & 1;
+      ok = wait_all(bar_full(st), (step / kStages) & 1, 210 + st);
+      if (ok && step >= 2) ok = wait_all(bar_tempty(buf), ((step >> 1) - 1) & 1, 200 + buf);
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t dw = desc_kmajor(base + st * L::kStageBytes), dx = desc_kmajor(base + st * L::kStageBytes + kABytes);
+#pragma unroll
+        for (int k = 0; k < kBK / 32; ++k) mma_f8(tmem_u + buf * NB, dw + 2 * k, dx + 2 * k, idesc, k > 0);
+        tc_commit(bar_tfull(buf));
+        tc_commit(bar_empty(st));
+      }
+    }
+    if (!ok) {
+      // drain the tensor pipe before TMEM is released
+      if (leader) tc_commit(bar_drain);
+      if (lane == 0)
+        for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_drain, 0); ++it) __nanosleep(64);
+      __syncwarp();
+    }
+  } else if (warp < 4) {
+    // ======================= scaled sums =======================
+    const uint32_t taddr = tmem_base + ((uint32_t)(warp * 32) << 16);
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      const int buf = step & 1, slot = step % L::kAhead;
+      if (step % L::kGroup == 0) ok &= mbar_wait(bar_sfull(slot / L::kGroup), (step / L::kAhead) & 1, abort_flag, a.wait_limit_ns, 310);
+      ok &= mbar_wait(bar_tfull(buf), (step >> 1) & 1, abort_flag, a.wait_limit_ns, 300 + buf);
+      __syncwarp();
+      tc_fence_after();
+      const float* scales = reinterpret_cast<const float*>(base_ptr + L::kScaleOff + slot * L::kSlot);
+      const float sw = scales[NB];
+#pragma unroll
+      for (int q = 0; q < NB; q += 16) {
+        uint32_t p[16];
+        XDIT_TMEM_LD16(p, taddr + buf * NB + q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 sx = *reinterpret_cast<const float4*>(scales + q + i);
+          fma_pair(acc[q + i], acc[q + i + 1], p[i], p[i + 1], f2_pack(sx.x * sw, sx.y * sw));
+          fma_pair(acc[q + i + 2], acc[q + i + 3], p[i + 2], p[i + 3], f2_pack(sx.z * sw, sx.w * sw));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar_tempty(buf));
+        if (step % L::kGroup == L::kGroup - 1) mbar_arrive(bar_sempty(slot / L::kGroup));
+      }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  }
+
+  // ======================= epilogue =======================
+  // Rows [first, last) of the tile of x are this CTA's; without a split they are all of them.
+  const int share = NB / a.splits, first = split * share, last = first + share;
+  if (a.splits > 1) {
+    // every MMA of this CTA has read the ring by now: the summing warps have waited for all of them
+    if (warp < 4) {
+      float* mine = reinterpret_cast<float*>(base_ptr);  // [128 rows of W][NB], rotated so that neighbours use other banks
+#pragma unroll
+      for (int i = 0; i < NB; i += 4)
+        *reinterpret_cast<float4*>(mine + (warp * 32 + lane) * NB + ((i + 4 * lane) & (NB - 1))) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    }
+    cluster_sync();
+  }
+  float y[NB];
+  if (warp < 4) {
+    if (a.splits > 1) {
+#pragma unroll
+      for (int i = 0; i < NB; i += 4) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i + 4 > first && i < last) {
+          const uint32_t at = base + ((warp * 32 + lane) * NB + ((i + 4 * lane) & (NB - 1))) * 4;
+          for (int c = 0; c < a.splits; ++c) {
+            const float4 u = load_cluster(at, c);
+            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+          }
+        }
+        y[i] = v.x; y[i + 1] = v.y; y[i + 2] = v.z; y[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) y[i] = acc[i];
     }
   }
+  if (a.splits > 1) cluster_sync();  // nobody leaves while its sums are being read
+  const int n = n0 + warp * 32 + lane;
+  if (warp < 4) {
+    const float bias = a.bias && n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      y[i] += bias;
+      if (a.act == XDIT_ACT_GELU_TANH) y[i] = gelu_tanh(y[i]);
+    }
+  }
+  if (a.out_q && !skip) {
+    // the tile's 128 columns of the result are one block: its rows' largest magnitudes over the four warps
+    float* tops = reinterpret_cast<float*>(base_ptr + L::kTopOff);
+    if (warp < 4) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, n < a.N ? __float_as_uint(fabsf(y[i])) : 0u);  // a NaN's bits are above an infinity's
+        if (lane == 0) tops[warp * NB + i] = __uint_as_float(top);
+      }
+    }
+    __syncthreads();
+    if (warp < 4 && ok) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int64_t m = m0 + i;
+        if (i < first || i >= last || m >= a.M) continue;
+        float inv;
+        const float top = amax_nan(amax_nan(tops[i], tops[NB + i]), amax_nan(tops[2 * NB + i], tops[3 * NB + i]));
+        const float sc = block_scale(top, inv);
+        if (n < a.N) a.out_q[m * a.N + n] = (uint8_t)pack_e4m3(y[i] * inv, 0.f, 0.f, 0.f);
+        if (threadIdx.x == 0) a.out_scale[(n0 / kBlock) * a.out_scale_ld + m] = sc;
+      }
+    }
+  } else if (warp < 4 && ok && n < a.N) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (i >= first && i < last && m0 + i < a.M) store_any(a.out, a.out_dtype, (int64_t)(m0 + i) * a.out_srow + n, y[i]);
+  }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmem) : "memory");
+  }
+  report(a, abort_flag);
 }
 
 // Map of a row-major matrix of `type`: boxes of `box_cols` by `box_rows`; what lies outside reads as zero and is not written.
@@ -442,6 +743,37 @@ int configure_smem(int bytes) {
   return XDIT_OK;
 }
 
+// Few rows: NB the smallest of 16, 32, 64 that holds them (tiles of 64 above), the K axis split while two CTAs per SM
+// are not reached and a CTA keeps four steps.
+template <int NB>
+int launch_rows(GemmArgs& a, const xdit_fp8_linear_params& p, int sms, bool after_quantise, cudaStream_t stream) {
+  using L = RowsLayout<NB>;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int rc;
+  if ((rc = encode_map(&a.tm_x, u8, 1, p.x, p.M, p.K, p.x_stride_row, NB, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  if ((rc = encode_map(&a.tm_w, u8, 1, p.w, p.N, p.K, p.w_stride_row, 128, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  const int nt = (p.N + 127) / 128, mt = (p.M + NB - 1) / NB;
+  a.splits = 1;
+  while (a.splits < 8 && (int64_t)nt * mt * a.splits * 2 <= 2 * sms && a.kb / (a.splits * 2) >= 4) a.splits *= 2;
+  if ((rc = configure_smem<fp8_rows_kernel<NB>>(L::kSmem))) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(nt * a.splits), (unsigned)mt);
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.splits;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = after_quantise ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_rows_kernel<NB>, a);
+  if (e != cudaSuccess) return cuda_fail(e, "fp8_rows_kernel launch");
+  return XDIT_OK;
+}
+
 }  // namespace
 }  // namespace xdit
 
@@ -464,6 +796,10 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
     set_error("%s: rows of x, w and out_q must start on 16-byte boundaries, out_scale_ld be at least M", who);
     return XDIT_E_ALIGN;
   }
+  if (p->raw && (p->x_scale_stride_row != 1 || p->x_stride_row != p->K || p->raw_s < 0 || (p->raw_s && p->M % p->raw_s))) {
+    set_error("%s: x is quantised into contiguous rows with scales stored block by block; raw_s=%d of M=%d", who, p->raw_s, p->M);
+    return XDIT_E_SHAPE;
+  }
   if (!p->out_q && (((uintptr_t)p->out) % es || (p->M > 1 && p->out_stride_row < p->N))) { set_error("%s: out pointer or row stride", who); return XDIT_E_ALIGN; }
   if (p->status_host) {
     const int32_t code = *reinterpret_cast<const volatile int32_t*>(p->status_host);
@@ -476,11 +812,15 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   int sms = 0;
   int rc = check_device(&sms);
   if (rc) return rc;
+  const bool quantise = p->raw != nullptr;
+  if (quantise) {
+    rc = launch_quantize_rows(who, p->raw, p->raw_stride_b, p->raw_stride_row, p->raw_dtype, p->raw_s ? p->M / p->raw_s : 1,
+                              p->raw_s ? p->raw_s : p->M, p->K, const_cast<void*>(p->x), const_cast<float*>(p->x_scale),
+                              p->x_scale_stride_block, stream);
+    if (rc) return rc;
+  }
   GemmArgs a;
   memset(&a, 0, sizeof(a));
-  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
-  if ((rc = encode_map(&a.tm_x, u8, 1, p->x, p->M, p->K, p->x_stride_row, kBM, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-  if ((rc = encode_map(&a.tm_w, u8, 1, p->w, p->N, p->K, p->w_stride_row, kBN, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   a.M = p->M; a.N = p->N;
   a.kb = (p->K + kBK - 1) / kBK;
   a.mt = (p->M + kBM - 1) / kBM;
@@ -491,14 +831,22 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   a.out = p->out; a.out_srow = p->out_stride_row;
   a.out_q = (uint8_t*)p->out_q; a.out_scale = p->out_scale; a.out_scale_ld = p->out_scale_ld;
   a.wide = ((uintptr_t)p->out) % 16 == 0 && (p->M == 1 || (p->out_stride_row * es) % 16 == 0);
+  a.status = p->status; a.status_host = p->status_host;
+  a.wait_limit_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
+  if (p->M <= 64) {
+    if (p->M <= 16) return launch_rows<16>(a, *p, sms, quantise, (cudaStream_t)stream);
+    if (p->M <= 32) return launch_rows<32>(a, *p, sms, quantise, (cudaStream_t)stream);
+    return launch_rows<64>(a, *p, sms, quantise, (cudaStream_t)stream);
+  }
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  if ((rc = encode_map(&a.tm_x, u8, 1, p->x, p->M, p->K, p->x_stride_row, kBM, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  if ((rc = encode_map(&a.tm_w, u8, 1, p->w, p->N, p->K, p->w_stride_row, kBN, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   a.tma_out = p->out_q || (a.wide && es == 2);
   if (p->out_q)
     rc = encode_map(&a.tm_out, u8, 1, p->out_q, p->M, p->N, p->N, 32, kCols, CU_TENSOR_MAP_SWIZZLE_64B);
   else if (a.tma_out)
     rc = encode_map(&a.tm_out, u16, 2, p->out, p->M, p->N, p->out_stride_row, 32, kCols, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  a.status = p->status; a.status_host = p->status_host;
-  a.wait_limit_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
   const int64_t tiles = (int64_t)a.mt * a.nt;
   if (tiles > 0x3fffffffll) { set_error("%s: too many tiles", who); return XDIT_E_SHAPE; }
   if ((rc = configure_smem<fp8_gemm_kernel>(kSmem))) return rc;

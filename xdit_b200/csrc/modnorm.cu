@@ -355,6 +355,8 @@ template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
 quantize_rows_kernel(const T* x, int64_t sb, int64_t srow, int s, int64_t rows, int K, uint8_t* q, float* scale,
                      int64_t ld) {
+  // a product that takes these rows may be launched now: it waits for this kernel's end before it reads them
+  asm volatile("griddepcontrol.launch_dependents;");
   constexpr int kUnroll = 4;
   const int nvec = K / 8, t = threadIdx.x;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -550,20 +552,8 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
   return XDIT_OK;
 }
 
-}  // namespace xdit
-
-using namespace xdit;
-
-extern "C" {
-
-int xdit_gated_residual_norm(const struct xdit_norm_params* p, void* stream) {
-  if (!p) { set_error("xdit_gated_residual_norm: NULL params"); return XDIT_E_NULL; }
-  return launch_norm(*p, (cudaStream_t)stream);
-}
-
-int xdit_quantize_rows(const void* x, int64_t stride_b, int64_t stride_row, int32_t dtype, int32_t B, int32_t s,
-                       int32_t K, void* q, float* scale, int64_t scale_ld, void* stream) {
-  const char* who = "xdit_quantize_rows";
+int launch_quantize_rows(const char* who, const void* x, int64_t stride_b, int64_t stride_row, int32_t dtype, int32_t B,
+                         int32_t s, int32_t K, void* q, float* scale, int64_t scale_ld, void* stream) {
   const int es = dtype_size(dtype);
   if (!es) { set_error("%s: bad dtype %d", who, dtype); return XDIT_E_DTYPE; }
   const int64_t rows = (int64_t)B * s;
@@ -590,6 +580,23 @@ int xdit_quantize_rows(const void* x, int64_t stride_b, int64_t stride_row, int3
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "quantize_rows_kernel launch");
   return XDIT_OK;
+}
+
+
+}  // namespace xdit
+
+using namespace xdit;
+
+extern "C" {
+
+int xdit_gated_residual_norm(const struct xdit_norm_params* p, void* stream) {
+  if (!p) { set_error("xdit_gated_residual_norm: NULL params"); return XDIT_E_NULL; }
+  return launch_norm(*p, (cudaStream_t)stream);
+}
+
+int xdit_quantize_rows(const void* x, int64_t stride_b, int64_t stride_row, int32_t dtype, int32_t B, int32_t s,
+                       int32_t K, void* q, float* scale, int64_t scale_ld, void* stream) {
+  return launch_quantize_rows("xdit_quantize_rows", x, stride_b, stride_row, dtype, B, s, K, q, scale, scale_ld, stream);
 }
 
 int xdit_quantize_weight(const void* w, int64_t stride_row, int32_t dtype, int32_t N, int32_t K, void* q, float* scale,

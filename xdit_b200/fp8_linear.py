@@ -57,20 +57,24 @@ def fp8_linear(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optiona
                quantize_out: bool = False) -> Union[torch.Tensor, Fp8Rows]:
     """``activation(x @ weight.T + bias)`` -> ``[..., N]``.
 
-    ``x``: a tensor ``[..., K]``, quantised here by :func:`quantize_rows`, or :class:`Fp8Rows` with scales of any value.
+    ``x``: a tensor ``[..., K]``, quantised by the rule of :func:`quantize_rows`, or :class:`Fp8Rows` with scales of any value.
     ``activation``: ``None`` or ``"gelu_tanh"``.  ``out_dtype``: bf16, fp16 or fp32 (the dtype of ``x`` when it is a tensor, else
     bf16).  ``quantize_out``: the result as :class:`Fp8Rows` (N a multiple of 16), quantised from the fp32 sums.  The sums of
     a block of 128 run in the tensor cores in fp32, their scaled sum in fp32 registers."""
+    w, ws = weight.data, weight.scale
     if isinstance(x, torch.Tensor):
         out_dtype = x.dtype if out_dtype is None else out_dtype
-        x = quantize_rows(x)
-    elif out_dtype is None:
-        out_dtype = torch.bfloat16
-    lead, M, N = x.shape[:-1], x.data.shape[0], weight.data.shape[0]
+        lead = x.shape[:-1]
+        data, scale = x if x.dim() == 3 else x.unsqueeze(0) if x.dim() == 2 else x.reshape(1, -1, x.shape[-1]), None
+        M = data.shape[0] * data.shape[1]
+    else:
+        out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        lead, data, scale = x.shape[:-1], x.data, x.scale
+        M = data.shape[0]
     if quantize_out:
-        data, scale = ops.empty_fp8_rows(M, N, x.data.device)
-        ops.fp8_linear(x.data, x.scale, weight.data, weight.scale, bias, activation=activation, out_q=data, out_scale=scale)
-        return Fp8Rows(data, scale, lead)
-    out = torch.empty(M, N, dtype=out_dtype, device=x.data.device)
-    ops.fp8_linear(x.data, x.scale, weight.data, weight.scale, bias, activation=activation, out=out)
-    return out.view(*lead, N)
+        q, s = ops.empty_fp8_rows(M, w.shape[0], data.device)
+        ops.fp8_linear(data, scale, w, ws, bias, activation=activation, out_q=q, out_scale=s)
+        return Fp8Rows(q, s, tuple(lead))
+    out = torch.empty(M, w.shape[0], dtype=out_dtype, device=data.device)
+    ops.fp8_linear(data, scale, w, ws, bias, activation=activation, out=out)
+    return out if len(lead) == 1 else out.view(*lead, w.shape[0])

@@ -79,7 +79,7 @@ def _device_index(device) -> int:
 
 
 def _status(device) -> _Status:
-    key = _device_index(device)
+    key = device.index if isinstance(device, torch.device) and device.index is not None else _device_index(device)
     st = _status_bufs.get(key)
     if st is None:
         st = _status_bufs[key] = _Status(key)
@@ -188,8 +188,12 @@ def attn_split_scratch_bytes(q, k, v, k2=None, v2=None) -> int:
 def _launch_attn(fn, p, q, where):
     """Call an attention entry point; a timeout reported by an earlier launch surfaces here, and the
     status words are cleared so that the caller may retry."""
-    with torch.cuda.device(q.device):
-        rc = fn(C.byref(p), _stream(q))
+    device = q.get_device()
+    if device == torch._C._cuda_getDevice():
+        rc = fn(C.byref(p), torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(C.byref(p), torch._C._cuda_getCurrentRawStream(device))
     if rc == -6:  # XDIT_E_KERNEL_TIMEOUT
         msg = _capi.load().xdit_last_error_string()
         torch.cuda.synchronize(q.device)
@@ -576,16 +580,31 @@ def qk_norm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: 
     launch_count += 1
 
 
-def _refuse_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _check_tensors(first: torch.Tensor, *others) -> None:
+    """What every launch asks of its tensors: no gradient to record, CUDA memory, one device."""
+    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
         raise NotImplementedError("backward passes are not part of this inference path: call it under "
                                   "torch.no_grad(), or with tensors that do not require a gradient")
-
-
-def _one_device(first: torch.Tensor, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != first.device:
+    if not first.is_cuda:
+        _require_cuda(first)
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            _require_cuda(t)
             raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+
+
+def _launch(fn, t: torch.Tensor, where: str, *args) -> None:
+    """``fn(*args, stream)`` on ``t``'s device and its current stream.  (The plain calls behind
+    ``torch.cuda.current_device`` and ``current_stream``: a launch of a few microseconds should not wait for more.)"""
+    device = t.get_device()
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _capi.check(rc, where)
 
 
 def _rows_contiguous(t: torch.Tensor, name: str) -> None:
@@ -628,30 +647,30 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.Rot
     """Rotate ``q`` [B, H, s, D] and ``k`` [B, Hk, s, D] by the angles of ``positions`` (:func:`rotary_positions`) into
     ``out_q`` and ``out_k``, which may be ``q`` and ``k`` themselves (``xdit_rotary_axes``)."""
     global launch_count
-    p = _capi.RotaryParams(dtype=_dtype(q), halves=int(bool(halves)), pos=positions)
-    p.B, p.H, p.s, p.D = q.shape
-    p.q, p.out_q = q.data_ptr(), out_q.data_ptr()
-    pairs = [(q, out_q, "q")]
+    B, H, s, D = q.shape
+    dtype = _dtype(q)
+    if out_q.dtype != q.dtype or (k is not None and (k.dtype != q.dtype or out_k.dtype != q.dtype)):
+        raise TypeError("q, k and their outputs must share one dtype")
+    if out_q.shape != q.shape or (k is not None and (k.shape != (B, k.shape[1], s, D) or out_k.shape != k.shape)):
+        raise ValueError("q, k and their outputs must agree in B, s and D")
+    if 2 * positions.pairs > D:
+        raise ValueError(f"{2 * positions.pairs} elements to rotate in a head of {D}")
+    qb, qh, qs, q1 = q.stride()
+    ob, oh, os_, o1 = out_q.stride()
+    kb = kh = ks = pb = ph = ps = Hk = 0
+    k_ptr = out_k_ptr = None
+    k1 = p1 = 1
     if k is not None:
-        p.Hk = k.shape[1]
-        p.k, p.out_k = k.data_ptr(), out_k.data_ptr()
-        pairs.append((k, out_k, "k"))
-    for i, (t, o, name) in enumerate(pairs):
-        if t.dtype != q.dtype or o.dtype != q.dtype:
-            raise TypeError("q, k and their outputs must share one dtype")
-        if o.shape != t.shape or t.shape[0] != p.B or t.shape[2] != p.s or t.shape[3] != p.D:
-            raise ValueError("q, k and their outputs must agree in B, s and D")
-        _rows_contiguous(t, name)
-        _rows_contiguous(o, "out_" + name)
-        p.stride_b[i], p.stride_h[i], p.stride_row[i] = t.stride(0), t.stride(1), t.stride(2)
-        p.out_stride_b[i], p.out_stride_h[i], p.out_stride_row[i] = o.stride(0), o.stride(1), o.stride(2)
-    if 2 * positions.pairs > p.D:
-        raise ValueError(f"{2 * positions.pairs} elements to rotate in a head of {p.D}")
-    _refuse_grad(q, k)
-    _require_cuda(q, k, out_q, out_k)
-    _one_device(q, k, out_q, out_k)
-    with torch.cuda.device(q.device):
-        _capi.check(_capi.load().xdit_rotary_axes(C.byref(p), _stream(q)), "xdit_rotary_axes")
+        Hk, k_ptr, out_k_ptr = k.shape[1], k.data_ptr(), out_k.data_ptr()
+        kb, kh, ks, k1 = k.stride()
+        pb, ph, ps, p1 = out_k.stride()
+    if D != 1 and (q1 != 1 or o1 != 1 or k1 != 1 or p1 != 1):
+        raise ValueError("the last axis of q, k and their outputs must be contiguous")
+    _check_tensors(q, k, out_q, out_k)
+    pair = C.c_int64 * 2
+    p = _capi.RotaryParams(dtype, B, H, Hk, s, D, halves, positions, q.data_ptr(), k_ptr, out_q.data_ptr(), out_k_ptr,
+                           pair(qb, kb), pair(qh, kh), pair(qs, ks), pair(ob, pb), pair(oh, ph), pair(os_, ps))
+    _launch(_capi.load().xdit_rotary_axes, q, "xdit_rotary_axes", C.byref(p))
     launch_count += 1
 
 
@@ -663,9 +682,8 @@ def rotary_tables(positions: _capi.RotaryPositions, s: int, D: int, device) -> t
     if device.type != "cuda":
         raise RuntimeError(f"xdit_b200 kernels run on CUDA devices only (sm_100a), not on {device}. There is no CPU fallback.")
     cos, sin = (torch.empty(s, D, dtype=torch.float32, device=device) for _ in range(2))
-    with torch.cuda.device(device):
-        _capi.check(_capi.load().xdit_rotary_tables(C.byref(positions), cos.data_ptr(), sin.data_ptr(), s, D,
-                                                    _stream(cos)), "xdit_rotary_tables")
+    _launch(_capi.load().xdit_rotary_tables, cos, "xdit_rotary_tables", C.byref(positions), cos.data_ptr(),
+            sin.data_ptr(), s, D)
     launch_count += 1
     return cos, sin
 
@@ -673,21 +691,41 @@ def rotary_tables(positions: _capi.RotaryPositions, s: int, D: int, device) -> t
 _NORMS = {None: _capi.XDIT_NORM_NONE, "layer": _capi.XDIT_NORM_LAYER, "rms": _capi.XDIT_NORM_RMS}
 
 
-def _row_vec(t: Optional[torch.Tensor], x: torch.Tensor, name: str, shared: bool = False) -> _capi.RowVec:
-    """A modulation row of ``x`` [B, s, C]: ``[C]``, ``[B or 1, C]`` or ``[B or 1, s or 1, C]``."""
+def _row_vec(t: Optional[torch.Tensor], x: torch.Tensor, name: str, shared: bool = False) -> tuple:
+    """A modulation row of ``x`` [B, s, C] as the fields of ``xdit_row_vec``: ``[C]``, ``[B or 1, C]`` or ``[B or 1, s or 1, C]``."""
     if t is None:
-        return _capi.RowVec()
+        return _NO_ROW
     B, s, Cn = x.shape
-    if t.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"{name} must be {x.dtype} or fp32, not {t.dtype}")
-    shape = t.shape if t.dim() == 3 else (t.shape[0], 1, t.shape[1]) if t.dim() == 2 else (1, 1) + tuple(t.shape)
-    if len(shape) != 3 or shape[0] not in (1, B) or shape[1] not in (1, s) or shape[2] != Cn or (shared and t.dim() != 1):
-        raise ValueError(f"{name} of shape {tuple(t.shape)} for rows of shape {tuple(x.shape)}")
-    _rows_contiguous(t, name)
-    v = _capi.RowVec(ptr=t.data_ptr(), dtype=_dtype(t))
-    v.stride_b = t.stride(0) if t.dim() > 1 and shape[0] > 1 else 0
-    v.stride_row = t.stride(1) if t.dim() == 3 and shape[1] > 1 else 0
-    return v
+    dtype = t.dtype
+    if dtype is not x.dtype and dtype is not torch.float32:
+        raise TypeError(f"{name} must be {x.dtype} or fp32, not {dtype}")
+    shape, stride = t.shape, t.stride()
+    n = len(shape)
+    sb = stride[0] if n > 1 and shape[0] != 1 else 0
+    srow = stride[1] if n == 3 and shape[1] != 1 else 0
+    if (not 1 <= n <= 3 or shape[-1] != Cn or (shared and n != 1) or (n > 1 and shape[0] != 1 and shape[0] != B)
+            or (n == 3 and shape[1] != 1 and shape[1] != s)):
+        raise ValueError(f"{name} of shape {tuple(shape)} for rows of shape {tuple(x.shape)}")
+    if stride[-1] != 1 and Cn != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+    return t.data_ptr(), sb, srow, _DTYPES[dtype]
+
+
+_NO_ROW = (None, 0, 0, 0)
+
+
+def _rows(t: Optional[torch.Tensor], x: torch.Tensor, name: str) -> tuple:
+    """``(address, batch stride, row stride)`` of a tensor shaped like ``x`` [B, s, C]."""
+    if t is None:
+        return None, 0, 0
+    if t.shape != x.shape:
+        raise ValueError(f"{name} {tuple(t.shape)} beside a residual {tuple(x.shape)}")
+    if t.dtype is not x.dtype:
+        raise TypeError(f"{name} must have the residual's dtype")
+    sb, srow, s1 = t.stride()
+    if s1 != 1 and x.shape[2] != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+    return t.data_ptr(), sb, srow
 
 
 def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], *, out_residual=None, out=None,
@@ -702,40 +740,25 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], 
         raise ValueError("expected [B, s, C]")
     if norm not in _NORMS or post_norm not in _NORMS:
         raise ValueError("a norm is None, 'layer' or 'rms'")
-    if norm is None and any(t is not None for t in (weight, bias, scale, shift)):
+    if norm is None and (weight is not None or bias is not None or scale is not None or shift is not None):
         raise ValueError("weight, bias, scale and shift need a norm")
     if branch is None and (post_norm is not None or gate is not None):
         raise ValueError("gate and post_norm need a branch")
     if post_norm is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias need a post_norm")
-    p = _capi.NormParams(dtype=_dtype(residual), post_norm=_NORMS[post_norm], norm=_NORMS[norm],
-                         residual_scale=float(residual_scale), eps=float(eps))
-    p.B, p.s, p.C = residual.shape
-    for name, t in (("residual", residual), ("branch", branch), ("out_residual", out_residual), ("out", out)):
-        if t is None:
-            continue
-        if t.shape != residual.shape:
-            raise ValueError(f"{name} {tuple(t.shape)} beside a residual {tuple(residual.shape)}")
-        if t.dtype != residual.dtype:
-            raise TypeError(f"{name} must have the residual's dtype")
-        _rows_contiguous(t, name)
-        setattr(p, name, t.data_ptr())
-        setattr(p, name + "_stride_b", t.stride(0))
-        setattr(p, name + "_stride_row", t.stride(1))
-    if out_q is not None:
-        p.out_q, p.out_scale, p.out_scale_ld = out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("weight", weight), ("bias", bias)):
-        if t is not None:
-            setattr(p, name, _row_vec(t, residual, name, shared=True))
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
-        if t is not None:
-            setattr(p, name, _row_vec(t, residual, name))
-    every = (branch, out_residual, out, out_q, out_scale, gate, post_weight, post_bias, weight, bias, scale, shift)
-    _refuse_grad(residual, *every)
-    _require_cuda(residual, *every)
-    _one_device(residual, *every)
-    with torch.cuda.device(residual.device):
-        _capi.check(_capi.load().xdit_gated_residual_norm(C.byref(p), _stream(residual)), "xdit_gated_residual_norm")
+    x = residual
+    dtype = _dtype(x)
+    B, s, Cn = x.shape
+    r, y = _rows(x, x, "residual"), _rows(branch, x, "branch")
+    oh, oz = _rows(out_residual, x, "out_residual"), _rows(out, x, "out")
+    rows = (_row_vec(post_weight, x, "post_weight", True), _row_vec(post_bias, x, "post_bias", True),
+            _row_vec(gate, x, "gate"), _row_vec(weight, x, "weight", True), _row_vec(bias, x, "bias", True),
+            _row_vec(scale, x, "scale"), _row_vec(shift, x, "shift"))
+    _check_tensors(x, branch, out_residual, out, out_q, out_scale, gate, post_weight, post_bias, weight, bias, scale, shift)
+    q = (out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)) if out_q is not None else (None, None, 0)
+    p = _capi.NormParams(dtype, B, s, Cn, _NORMS[post_norm], _NORMS[norm], residual_scale, eps, r[0], y[0], r[1], r[2],
+                         y[1], y[2], oh[0], oz[0], oh[1], oh[2], oz[1], oz[2], *q, *rows)
+    _launch(_capi.load().xdit_gated_residual_norm, x, "xdit_gated_residual_norm", C.byref(p))
     launch_count += 1
 
 
@@ -765,13 +788,10 @@ def quantize_rows(x: torch.Tensor) -> tuple:
         raise ValueError(f"rows of {K} values: a multiple of 16 is needed")
     dt = _dtype(x)
     _rows_contiguous(x, "x")
-    _refuse_grad(x)
-    _require_cuda(x)
+    _check_tensors(x)
     data, scale = empty_fp8_rows(B * s, K, x.device)
-    with torch.cuda.device(x.device):
-        _capi.check(_capi.load().xdit_quantize_rows(x.data_ptr(), x.stride(0), x.stride(1), dt, B, s, K,
-                                                    data.data_ptr(), scale.data_ptr(), _scale_ld(scale), _stream(x)),
-                    "xdit_quantize_rows")
+    _launch(_capi.load().xdit_quantize_rows, x, "xdit_quantize_rows", x.data_ptr(), x.stride(0), x.stride(1), dt, B, s, K,
+            data.data_ptr(), scale.data_ptr(), _scale_ld(scale))
     launch_count += 1
     return data, scale
 
@@ -784,15 +804,13 @@ def quantize_weight(w: torch.Tensor) -> tuple:
         raise ValueError(f"a weight [N, K] with K a multiple of 16 is needed, got {tuple(w.shape)}")
     dt = _dtype(w)
     _rows_contiguous(w, "w")
-    _refuse_grad(w)
-    _require_cuda(w)
+    _check_tensors(w)
     N, K = w.shape
     data = torch.empty(N, K, dtype=torch.float8_e4m3fn, device=w.device)
     b = _capi.XDIT_FP8_BLOCK
     scale = torch.empty(-(-N // b), -(-K // b), dtype=torch.float32, device=w.device)
-    with torch.cuda.device(w.device):
-        _capi.check(_capi.load().xdit_quantize_weight(w.data_ptr(), w.stride(0), dt, N, K, data.data_ptr(),
-                                                      scale.data_ptr(), _stream(w)), "xdit_quantize_weight")
+    _launch(_capi.load().xdit_quantize_weight, w, "xdit_quantize_weight", w.data_ptr(), w.stride(0), dt, N, K,
+            data.data_ptr(), scale.data_ptr())
     launch_count += 1
     return data, scale
 
@@ -800,57 +818,69 @@ def quantize_weight(w: torch.Tensor) -> tuple:
 _ACTIVATIONS = {None: _capi.XDIT_ACT_NONE, "gelu_tanh": _capi.XDIT_ACT_GELU_TANH}
 
 
-def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor, w_scale: torch.Tensor,
                bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
                out: Optional[torch.Tensor] = None, out_q: Optional[torch.Tensor] = None,
                out_scale: Optional[torch.Tensor] = None, _wait_limit_ns: int = 0) -> None:
-    """``out = act(x w^T + bias)`` of e4m3 rows ``x`` [M, K] and a weight ``w`` [N, K] with fp32 scales ``x_scale`` [M, K/128] and
-    ``w_scale`` [N/128, K/128] of any value and strides (``xdit_fp8_linear``).  ``out`` [M, N] in bf16, fp16 or fp32, or ``out_q``
-    with ``out_scale`` for e4m3 rows again."""
+    """``out = act(x w^T + bias)`` with a weight ``w`` [N, K] in e4m3 and fp32 scales ``w_scale`` [N/128, K/128] of any value and
+    strides (``xdit_fp8_linear``).  ``x``: e4m3 rows [M, K] with ``x_scale`` [M, K/128]; or, with ``x_scale`` ``None``, a bf16, fp16
+    or fp32 tensor [B, s, K] that is quantised first (M = B*s).  ``out`` [M, N] in bf16, fp16 or fp32, or ``out_q`` with
+    ``out_scale`` for e4m3 rows again."""
     global launch_count
-    b = _capi.XDIT_FP8_BLOCK
-    if x.dtype != torch.float8_e4m3fn or w.dtype != torch.float8_e4m3fn:
+    given = x_scale is not None
+    if w.dtype is not torch.float8_e4m3fn or (given and x.dtype is not torch.float8_e4m3fn):
         raise TypeError("x and w must be float8_e4m3fn")
-    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+    if w_scale.dtype is not torch.float32 or (given and x_scale.dtype is not torch.float32):
         raise TypeError("the scales must be fp32")
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+    if x.dim() != (2 if given else 3) or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"rows {tuple(x.shape)} and a weight {tuple(w.shape)}")
-    M, K = x.shape
-    N = w.shape[0]
+    N, K = w.shape
+    M = x.shape[0] if given else x.shape[0] * x.shape[1]
     if K % 16 or K == 0 or N == 0:
         raise ValueError(f"K = {K}: a multiple of 16 is needed (and N = {N} rows of the weight)")
-    if tuple(x_scale.shape) != (M, -(-K // b)) or tuple(w_scale.shape) != (-(-N // b), -(-K // b)):
-        raise ValueError(f"scales {tuple(x_scale.shape)} and {tuple(w_scale.shape)} for rows {tuple(x.shape)} and a weight {tuple(w.shape)}")
+    kb, nb = (K + 127) // 128, (N + 127) // 128
+    if w_scale.shape != (nb, kb) or (given and x_scale.shape != (M, kb)):
+        raise ValueError(f"scales of other shapes than {(M, kb)} and {(nb, kb)} for rows {tuple(x.shape)} and a weight {tuple(w.shape)}")
     if activation not in _ACTIVATIONS:
         raise ValueError("an activation is None or 'gelu_tanh'")
-    if bias is not None and (tuple(bias.shape) != (N,) or (bias.stride(0) != 1 and N > 1)):
+    if bias is not None and (bias.shape != (N,) or (bias.stride(0) != 1 and N > 1)):
         raise ValueError(f"a contiguous bias of {N} values is needed")
     if (out is None) == (out_q is None):
         raise ValueError("give either out or out_q")
-    p = _capi.Fp8LinearParams(M=M, N=N, K=K, activation=_ACTIVATIONS[activation])
+    ws0, ws1 = w.stride()
+    xs = x.stride()
+    if (ws1 != 1 or xs[-1] != 1) and K != 1:
+        raise ValueError("the last axis of x and w must be contiguous")
+    o = (None, 0, None, None, 0)
+    out_dtype = 0
     if out is not None:
-        if tuple(out.shape) != (M, N):
+        if out.shape != (M, N):
             raise ValueError(f"out {tuple(out.shape)} for a result of {(M, N)}")
         _rows_contiguous(out, "out")
-        p.out_dtype, p.out, p.out_stride_row = _dtype(out), out.data_ptr(), out.stride(0)
+        out_dtype = _dtype(out)
+        o = (out.data_ptr(), out.stride(0), None, None, 0)
     else:
         if N % 16:
             raise ValueError(f"e4m3 rows of {N} values: a multiple of 16 is needed")
-        p.out_q, p.out_scale, p.out_scale_ld = out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)
-    for t, name in ((x, "x"), (w, "w")):
-        _rows_contiguous(t, name)
-    p.x, p.x_stride_row, p.w, p.w_stride_row = x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0)
-    p.x_scale, p.x_scale_stride_row, p.x_scale_stride_block = x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1)
-    p.w_scale, p.w_scale_stride_row, p.w_scale_stride_block = w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1)
-    if bias is not None:
-        p.bias, p.bias_dtype = bias.data_ptr(), _dtype(bias)
-    _refuse_grad(bias)
-    _require_cuda(x, x_scale, w, w_scale, bias, out, out_q, out_scale)
-    _one_device(x, x_scale, w, w_scale, bias, out, out_q, out_scale)
+        o = (None, 0, out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale))
+    b = (bias.data_ptr(), _dtype(bias)) if bias is not None else (None, 0)
+    raw = (0, 0, None, 0, 0)
+    if not given:
+        raw = (_dtype(x), x.shape[1], x.data_ptr(), xs[0], xs[1])
+    _check_tensors(x, x_scale, w, w_scale, bias, out, out_q, out_scale)
+    if given:
+        rows, scales, (scale_row, scale_block) = x, x_scale, x_scale.stride()
+    else:  # e4m3 rows and behind them their scales, block by block
+        rows = torch.empty((M * K + 15) // 16 * 16 + 4 * M * kb, dtype=torch.uint8, device=x.device)
+        scale_row, scale_block = 1, M
+    address = rows.data_ptr()
     st = _status(x.device)
-    p.status, p.status_host, p.wait_limit_ns = st.dev.data_ptr(), st.host.data_ptr(), int(_wait_limit_ns)
+    p = _capi.Fp8LinearParams(M, N, K, _ACTIVATIONS[activation], out_dtype, b[1], address, w.data_ptr(), xs[0] if given else K,
+                              ws0, scales.data_ptr() if given else address + (M * K + 15) // 16 * 16, w_scale.data_ptr(),
+                              scale_row, scale_block, *w_scale.stride(), b[0], *o, st.dev.data_ptr(), st.host.data_ptr(),
+                              _wait_limit_ns, *raw)
     _launch_attn(_capi.load().xdit_fp8_linear, p, x, "xdit_fp8_linear")
-    launch_count += 1
+    launch_count += 1 if given else 2
 
 
 def default_scale(D: int) -> float:

@@ -96,7 +96,7 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], embedding: Ro
         raise ValueError("out_key without a key")
     p = embedding._params(query.shape[0], query.shape[2])
     if embedding.positions is not None:
-        ops._one_device(query, embedding.positions)
+        ops._check_tensors(query, embedding.positions)
     out_query = torch.empty_like(query) if out_query is None else out_query
     if key is not None and out_key is None:
         out_key = torch.empty_like(key)
