@@ -4,19 +4,26 @@
 // The inner sums run on the tensor cores (tcgen05.mma kind::f8f6f4, fp32 accumulators in TMEM); the scales
 // differ from block to block, so every inner sum is taken out of TMEM, scaled and added in registers.
 //
-// One CTA per SM walks output tiles of 128 rows x 256 columns.  A step is one block of 128 along K, which
-// is also one 128-byte swizzle row of the operands in shared memory:
-//   warp 17      loads the step's operands by TMA (16 KB of x, 32 KB of W) into a ring
-//   warp 18      copies the step's scales (128 of x, 2 of W) into a ring of their own, up to 16 steps ahead: read
-//                when they are needed, they arrived later than the MMAs (780 against 705 cycles a step)
-//   warp 16      issues the step's four MMAs (128 x 256 x 32) into one of two TMEM buffers of 256 columns
-//   warps 0-15   four warpgroups, 64 columns each: thread = row, 64 fp32 sums in registers; they add the scaled
-//                buffer of one step while the tensor core fills the other.  Four warps a scheduler keep its FMA
-//                pipe busier than two with 128 sums each (705 against 810 cycles); the MMAs alone take 595.
+// A CTA holds 128 rows of x by 256 columns of sums; a pair of CTAs (a cluster, tcgen05 cta_group::2) shares a tile of 256
+// rows, each loading half of W's 256 rows, and few tiles go to single CTAs.  The CTAs are persistent, one on an SM.  A
+// step is one block of 128 along K, which is also one 128-byte swizzle row of the operands in shared memory:
+//   warp 9      loads the step's operands by TMA into a ring
+//   warp 10     copies the step's scales (128 of x, 2 of W) into a ring of their own, up to 16 steps ahead: read when they
+//               are needed, they arrive later than the MMAs
+//   warp 8      issues the step's four MMAs (K = 32 each) into one of two TMEM buffers of 256 columns
+//   warps 0-7   two warpgroups, one for each block of 128 columns: thread = row, 128 fp32 sums in registers; they add the
+//               scaled buffer of one step while the tensor core fills the other
 // After the last step the sums get bias and activation and are rounded once; they leave through shared memory and
 // TMA stores, which also clip the edges (16-byte stores from registers, 32 rows an instruction, cost a fifth of
-// the whole time).  Or they become e4m3 rows again: two warpgroups hold a block of 128 and exchange the rows'
-// largest magnitudes.
+// the whole time).  Or they become e4m3 rows again: a thread holds a whole block of its row.
+//
+// What bounds it: the MMAs alone take 533 cycles a step by pairs (595 by single CTAs; 512 is the tensor core's rate), the
+// scaled sums bring that to about 700.  They are 256 cycles of packed FMAs and the TMEM reads of two warps a scheduler,
+// and what counted was keeping the rest out of their way: scales copied ahead, the next 16 columns loaded while the
+// last ones are added, the buffer released before its last sums, arrivals without branches, the loop unrolled by
+// four (853 cycles without these).  Four warpgroups of 64 columns run out of registers (855).  Over seconds the power
+// limit sets the clock: 75,600 x 5120 x 15360 runs at 2.2-2.36 PFLOP/s and about 1.4 GHz, a library product with one scale
+// for everything at 2.6.
 //
 // Every wait on an mbarrier is bounded in time; when one gives up the CTA raises a flag in shared memory, all
 // roles leave their loops, outstanding copies and MMAs are drained with bounded waits, TMEM is freed and
@@ -30,24 +37,29 @@
 namespace xdit {
 namespace {
 
-constexpr int kThreads = 640;  // 16 summing warps, MMA warp, TMA warp, scale warp, 1 idle warp (full register-trading warpgroup)
+constexpr int kThreads = 384;  // 8 summing warps, MMA warp, TMA warp, scale warp, 1 idle warp (full register-trading warpgroup)
+constexpr int kSumWarps = 8;
 constexpr int kBM = 128, kBN = 256, kBK = XDIT_FP8_BLOCK;
-constexpr int kCols = 64;      // columns of a summing thread
-constexpr int kStages = 3;
+constexpr int kCols = 128;     // columns of a summing thread: those that share a scale of W
 constexpr int kAhead = 16;     // steps whose scales are in shared memory or on their way
-constexpr int kABytes = kBM * kBK, kBBytes = kBN * kBK, kStageBytes = kABytes + kBBytes;
-constexpr int kWarpOut = 32 * kCols * 2;                // staging of a summing warp's results
-constexpr int kOutOff = kStages * kStageBytes;
-constexpr int kBiasOff = kOutOff + 16 * kWarpOut;       // [16 warps][64 columns]
-constexpr int kScaleOff = kBiasOff + 16 * kCols * 4;    // [kAhead][128 rows of x + 2 of w, padded]
-constexpr int kScaleBytes = 576;
-constexpr int kTopOff = kScaleOff + kAhead * kScaleBytes;  // [2 turns][4 warpgroups][128 rows] largest magnitudes
-constexpr int kBarOff = kTopOff + 2 * 4 * 128 * 4;
 constexpr int kGroup = 4, kGroups = kAhead / kGroup;  // steps whose scales share a barrier
-constexpr int kNumBars = 2 * kStages + 4 + 1 + 2 * kGroups + 2;
-constexpr int kMiscOff = kBarOff + kNumBars * 8;
-constexpr int kSmem = kMiscOff + 16 + 1024;  // with slack to align the base to 1024 bytes
-constexpr int kBand = 16;                    // row tiles of a band: tiles of a band are walked column by column
+constexpr int kABytes = kBM * kBK;
+constexpr int kWarpOut = 32 * kCols * 2;  // staging of a summing warp's results
+constexpr int kScaleBytes = 576;          // 128 scales of x + 2 of w, padded
+constexpr int kBand = 2048;               // rows of a band: the tiles of a band are walked column by column
+
+template <bool PAIR> struct GemmLayout {
+  static constexpr int kStages = PAIR ? 4 : 3;
+  static constexpr int kBRows = PAIR ? kBN / 2 : kBN;        // rows of W that a CTA loads
+  static constexpr int kStageBytes = kABytes + kBRows * kBK;
+  static constexpr int kOutOff = kStages * kStageBytes;
+  static constexpr int kBiasOff = kOutOff + kSumWarps * kWarpOut;   // [8 warps][128 columns]
+  static constexpr int kScaleOff = kBiasOff + kSumWarps * kCols * 4;     // [kAhead]
+  static constexpr int kBarOff = kScaleOff + kAhead * kScaleBytes;
+  static constexpr int kNumBars = 2 * kStages + 4 + 1 + 2 * kGroups;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kSmem = kMiscOff + 16 + 1024;  // with slack to align the base to 1024 bytes
+};
 
 struct alignas(64) GemmArgs {
   CUtensorMap tm_x, tm_w, tm_out;
@@ -85,6 +97,44 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
       : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),   \
         "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15])                    \
       : "r"(taddr) : "memory")
+// The same load by one CTA of a pair, whose bytes are counted on a barrier of either CTA (`bar`: its address in the cluster).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrival on a barrier of a CTA of the cluster (`bar`: its address in the cluster).
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Arrival of the lanes that have `yes`, without a branch: one between a TMEM load and the sums that use it makes the
+// compiler move registers.
+template <bool CLUSTER>
+__device__ __forceinline__ void mbar_arrive_if(uint32_t bar, uint32_t yes) {
+  if constexpr (CLUSTER)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar), "r"(yes) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"(yes) : "memory");
+}
+// Completion of the MMAs issued so far, on the same barrier of both CTAs of a pair.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tm), "r"(src), "r"(c0), "r"(c1) : "memory");
 }
@@ -104,11 +154,18 @@ __device__ __forceinline__ uint32_t pack16(int dtype, float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+template <bool PAIR = false>
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == XDIT_F32) return __ldg(reinterpret_cast<const float*>(p) + i);
@@ -120,10 +177,27 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x
   else if (dtype == XDIT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
 }
-// x/2 (1 + tanh u) = x / (1 + exp(-2u)) with u = sqrt(2/pi) (x + 0.044715 x^3)
-__device__ __forceinline__ float gelu_tanh(float x) {
-  const float u = 0.7978845608028654f * fmaf(0.044715f * x * x, x, x);
-  return __fdividef(x, 1.f + __expf(-2.f * u));
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// x/2 (1 + tanh u) = x / (1 + exp(-2u)) with u = sqrt(2/pi) (x + 0.044715 x^3), for two values: the polynomial
+// -2u log2(e) on packed pairs, then base-2 exponentials and reciprocals (2^-22 off).
+__device__ __forceinline__ void gelu_tanh2(float& x0, float& x1) {
+  constexpr float k1 = -2.f * 0.7978845608028654f * 1.4426950408889634f, k3 = k1 * 0.044715f;
+  const uint64_t x = f2_pack(x0, x1);
+  const uint64_t z = f2_mul(x, f2_fma(f2_mul(x, x), f2_pack(k3, k3), f2_pack(k1, k1)));
+  float z0, z1;
+  f2_unpack(z, z0, z1);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(z0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(z1));
+  z0 += 1.f;
+  z1 += 1.f;
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(z0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(z1));
+  x0 *= z0;
+  x1 *= z1;
 }
 // A CTA whose wait gave up tells the later launches and the host.
 __device__ __forceinline__ void report(const GemmArgs& a, volatile int* abort_flag) {
@@ -135,18 +209,24 @@ __device__ __forceinline__ void report(const GemmArgs& a, volatile int* abort_fl
     }
   }
 }
+// Tile t: its first row and column of tiles, `rows` rows of x a tile.
+template <int ROWS>
 __device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& m, int& n) {
-  const int band = t / (kBand * a.nt), rem = t - band * kBand * a.nt;
-  const int rows = min(kBand, a.mt - band * kBand);
-  n = rem / rows;
-  m = band * kBand + rem - n * rows;
+  constexpr int kHigh = kBand / ROWS;
+  const int band = t / (kHigh * a.nt), rem = t - band * kHigh * a.nt;
+  const int high = min(kHigh, a.mt - band * kHigh);
+  n = rem / high;
+  m = band * kHigh + rem - n * high;
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_constant__ GemmArgs a) {
+  using L = GemmLayout<PAIR>;
+  constexpr int kStages = L::kStages, kRows = PAIR ? 2 * kBM : kBM;  // rows of a tile
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = smem_u32(smem_dyn), base = (raw + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_dyn + (base - raw);
-  const uint32_t bar0 = base + kBarOff;
+  const uint32_t bar0 = base + L::kBarOff;
   auto bar_full = [&](int s) { return bar0 + 8u * s; };
   auto bar_empty = [&](int s) { return bar0 + 8u * (kStages + s); };
   auto bar_tfull = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
@@ -154,71 +234,99 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
   const uint32_t bar_drain = bar0 + 8u * (2 * kStages + 4);
   auto bar_sfull = [&](int s) { return bar0 + 8u * (2 * kStages + 5 + s); };
   auto bar_sempty = [&](int s) { return bar0 + 8u * (2 * kStages + 5 + kGroups + s); };
-  auto bar_top = [&](int pair) { return bar0 + 8u * (2 * kStages + 5 + 2 * kGroups + pair); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kMiscOff);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + kMiscOff + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + L::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + L::kMiscOff + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = a.mt * a.nt;
+  // A pair of CTAs (a cluster) shares a tile: each holds its 128 rows of x and of the sums, and half of W's rows; the
+  // first one, `rank` 0, issues the MMAs of both.
+  const int rank = PAIR ? (int)cta_rank() : 0;
+  const int tile0 = PAIR ? blockIdx.x / 2 : blockIdx.x, tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(bar_tfull(s), 1); mbar_init(bar_tempty(s), 16); }
-    for (int s = 0; s < kGroups; ++s) { mbar_init(bar_sfull(s), 32); mbar_init(bar_sempty(s), 16); }
-    for (int s = 0; s < 2; ++s) mbar_init(bar_top(s), 8);
+    for (int s = 0; s < 2; ++s) { mbar_init(bar_tfull(s), 1); mbar_init(bar_tempty(s), PAIR ? 2 * kSumWarps : kSumWarps); }
+    for (int s = 0; s < kGroups; ++s) { mbar_init(bar_sfull(s), 32); mbar_init(bar_sempty(s), kSumWarps); }
     mbar_init(bar_drain, 1);
     *abort_flag = status_is_set(a.status) ? -1 : 0;  // -1: skip all work (an earlier failure is pending)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 16) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if (warp == 8) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const bool skip = *abort_flag != 0;  // same value for every thread: written before the barrier above
+  bool skip = *abort_flag != 0;  // same value for every thread: written before the barrier above
+  if constexpr (PAIR) {
+    // the other CTA's barriers are ready behind this, and both skip where one has seen a failure
+    cluster_sync();
+    uint32_t other;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(other) : "r"(map_to_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1)) : "memory");
+    skip |= other != 0;
+    cluster_sync();  // neither changes its flag before both have read them
+  }
 
   if (skip) {
     // nothing to do: fall through to the teardown, which frees TMEM
-  } else if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");  // per scheduler 4 x 112 + 32 = 5 x 96, what the launch holds
-    if (warp == 17) {
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");  // per scheduler 2 x 232 + 40 = 3 x 168, what the launch holds
+    if (warp == 9) {
       // ======================= TMA producer =======================
       if (lane == 0) {
         int issued = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (int t = tile0; t < tiles && ok; t += tile_step) {
           int m, n;
-          tile_at(a, t, m, n);
+          tile_at<kRows>(a, t, m, n);
           for (int c = 0; c < a.kb; ++c) {
             const int st = issued % kStages, turn = issued / kStages;
             if (turn > 0) ok = mbar_wait(bar_empty(st), (turn - 1) & 1, abort_flag, a.wait_limit_ns, 100 + st);
             if (!ok) break;
-            mbar_arrive_expect_tx(bar_full(st), kStageBytes);
-            tma_load_2d(base + st * kStageBytes, &a.tm_x, bar_full(st), c * kBK, m * kBM);
-            tma_load_2d(base + st * kStageBytes + kABytes, &a.tm_w, bar_full(st), c * kBK, n * kBN);
+            const uint32_t to = base + st * L::kStageBytes;
+            if constexpr (PAIR) {  // both CTAs' bytes count on the first one's barrier
+              if (rank == 0) mbar_arrive_expect_tx(bar_full(st), 2 * L::kStageBytes);
+              const uint32_t full = map_to_cta(bar_full(st), 0);
+              tma_load_2d_pair(to, &a.tm_x, full, c * kBK, m * kRows + rank * kBM);
+              tma_load_2d_pair(to + kABytes, &a.tm_w, full, c * kBK, n * kBN + rank * L::kBRows);
+            } else {
+              mbar_arrive_expect_tx(bar_full(st), L::kStageBytes);
+              tma_load_2d(to, &a.tm_x, bar_full(st), c * kBK, m * kBM);
+              tma_load_2d(to + kABytes, &a.tm_w, bar_full(st), c * kBK, n * kBN);
+            }
             ++issued;
           }
         }
+        if constexpr (PAIR) {
+          // the MMAs report the last stages' release to both CTAs: neither may leave before that has arrived
+          for (int i = issued > kStages ? issued - kStages : 0; i < issued && ok; ++i)
+            ok = mbar_wait(bar_empty(i % kStages), (i / kStages) & 1, abort_flag, a.wait_limit_ns, 110);
+        }
         if (!ok) {
-          // drain: every armed stage must have received its bytes before the CTA may leave
-          for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          // drain: every armed stage must have received its bytes before the CTA may leave (a pair: before either leaves)
+          for (int i = rank ? issued : issued > kStages ? issued - kStages : 0; i < issued; ++i)
             for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_full(i % kStages), (i / kStages) & 1); ++it) __nanosleep(64);
         }
       }
-    } else if (warp == 18) {
+    } else if (warp == 10) {
       // ======================= scales: each lane the rows lane, lane + 32, ... of the tile =======================
       // A load from L2 takes longer than a step, so they are copied asynchronously, up to kAhead steps ahead.
       int step = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = tile0; t < tiles && ok; t += tile_step) {
         int m, n;
-        tile_at(a, t, m, n);
+        tile_at<kRows>(a, t, m, n);
         const float* src[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = m * kBM + 32 * i + lane;  // rows and columns behind the end take any scale
+          const int row = m * kRows + rank * kBM + 32 * i + lane;  // rows and columns behind the end take any scale
           src[i] = a.xs + (int64_t)(row < a.M ? row : 0) * a.xs_srow;
         }
         const int nb = n * (kBN / kBK) + (lane & 1);
@@ -227,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
           const int slot = step % kAhead, turn = step / kAhead, group = slot / kGroup;
           if (turn > 0 && step % kGroup == 0) ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty(group), (turn - 1) & 1, abort_flag, a.wait_limit_ns, 320));
           if (!ok) break;
-          const uint32_t at = base + kScaleOff + slot * kScaleBytes + lane * 4;
+          const uint32_t at = base + L::kScaleOff + slot * kScaleBytes + lane * 4;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + 128 * i), "l"(src[i]) : "memory");
@@ -242,17 +350,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       if (step % kGroup)  // the last group is not full
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_sfull(step % kAhead / kGroup)) : "memory");
       asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == 16) {
+    } else if (warp == 8 && rank == 0) {
       // ======================= MMA issuer (the warp runs converged, one elected lane issues) =======================
       const bool leader = elect_one();
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-      const uint32_t idesc = (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> fp32
+      const uint32_t idesc = (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);  // e4m3 x e4m3 -> fp32
       bool ok = true;
       int step = 0;
       auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.wait_limit_ns, code));
       };
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = tile0; t < tiles && ok; t += tile_step) {
         for (int c = 0; c < a.kb; ++c, ++step) {
           const int st = step % kStages, buf = step & 1;
           ok = wait_all(bar_full(st), (step / kStages) & 1, 210 + st);
@@ -260,39 +368,45 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            const uint64_t da = desc_kmajor(base + st * kStageBytes), db = desc_kmajor(base + st * kStageBytes + kABytes);
+            const uint64_t da = desc_kmajor(base + st * L::kStageBytes), db = desc_kmajor(base + st * L::kStageBytes + kABytes);
 #pragma unroll
-            for (int k = 0; k < kBK / 32; ++k) mma_f8(tmem_u + buf * kBN, da + 2 * k, db + 2 * k, idesc, k > 0);
-            tc_commit(bar_tfull(buf));
-            tc_commit(bar_empty(st));
+            for (int k = 0; k < kBK / 32; ++k) mma_f8<PAIR>(tmem_u + buf * kBN, da + 2 * k, db + 2 * k, idesc, k > 0);
+            if constexpr (PAIR) {
+              tc_commit_pair(bar_tfull(buf));
+              tc_commit_pair(bar_empty(st));
+            } else {
+              tc_commit(bar_tfull(buf));
+              tc_commit(bar_empty(st));
+            }
           }
         }
       }
       if (!ok) {
         // drain the tensor pipe before TMEM is released
-        if (leader) tc_commit(bar_drain);
+        if (leader) {
+          if constexpr (PAIR) tc_commit_pair(bar_drain);
+          else tc_commit(bar_drain);
+        }
         if (lane == 0)
           for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_drain, 0); ++it) __nanosleep(64);
         __syncwarp();
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ======================= scaled sums + epilogue =======================
-    const int group = warp >> 2;  // columns [64 group, 64 group + 64) of the tile
+    const int group = warp >> 2;  // columns [128 group, 128 group + 128) of the tile
     const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + group * kCols;
-    const int row_in = (warp & 3) * 32 + lane;
-    const uint32_t scale_x = base + kScaleOff + row_in * 4, scale_w = base + kScaleOff + 512 + (group >> 1) * 4;
-    const uint32_t stage = base + kOutOff + warp * kWarpOut;
-    float* bias = reinterpret_cast<float*>(base_ptr + kBiasOff) + warp * kCols;
-    float* tops = reinterpret_cast<float*>(base_ptr + kTopOff);
+    const uint32_t scale_x = base + L::kScaleOff + ((warp & 3) * 32 + lane) * 4, scale_w = base + L::kScaleOff + 512 + group * 4;
+    const uint32_t tempty_at = PAIR ? map_to_cta(bar_tempty(0), 0) : bar_tempty(0);
     bool ok = true;
-    int step = 0, turn = 0;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++turn) {
-      int m, n;
-      tile_at(a, t, m, n);
-      const int row0 = m * kBM + (warp & 3) * 32, col0 = n * kBN + group * kCols;
+    int step = 0;
+    for (int t = tile0; t < tiles && ok; t += tile_step) {
       if (a.bias) {
+        int m, n;
+        tile_at<kRows>(a, t, m, n);
+        const int col0 = n * kBN + group * kCols;
+        float* bias = reinterpret_cast<float*>(base_ptr + L::kBiasOff) + warp * kCols;
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kCols; i += 32)
@@ -302,40 +416,47 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0;
-#pragma unroll 1
+#pragma unroll 4
       for (int c = 0; c < a.kb; ++c, ++step) {
         const int buf = step & 1, slot = step % kAhead;
         // no way out of this loop: with one, the compiler copies all sums in every step.  After a wait that gave
         // up, the others return at once.
         if (step % kGroup == 0) ok &= mbar_wait(bar_sfull(slot / kGroup), (step / kAhead) & 1, abort_flag, a.wait_limit_ns, 310);
-        float sx, sw;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sx) : "r"(scale_x + slot * kScaleBytes) : "memory");
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sw) : "r"(scale_w + slot * kScaleBytes) : "memory");
-        const uint64_t s2 = f2_pack(sx * sw, sx * sw);
         ok &= mbar_wait(bar_tfull(buf), (step >> 1) & 1, abort_flag, a.wait_limit_ns, 300 + buf);
         __syncwarp();
         tc_fence_after();
         const uint32_t tb = taddr + buf * kBN;
+        uint32_t p[2][16];
+        XDIT_TMEM_LD16(p[0], tb);
+        float sx, sw;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sx) : "r"(scale_x + slot * kScaleBytes) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sw) : "r"(scale_w + slot * kScaleBytes) : "memory");
+        const uint64_t s2 = f2_pack(sx * sw, sx * sw);
+        tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < kCols / 32; ++q) {
-          uint32_t p[32];
-          XDIT_TMEM_LD32(p, 0, tb + 32 * q);
-          tmem_wait_ld();
+        for (int q = 0; q < kCols; q += 16) {
+          const int h = (q >> 4) & 1;
+          if (q + 16 < kCols) XDIT_TMEM_LD16(p[h ^ 1], tb + q + 16);
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            fma_pair(acc[32 * q + 2 * i], acc[32 * q + 2 * i + 1], p[2 * i], p[2 * i + 1], s2);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar_tempty(buf));
-          if (step % kGroup == kGroup - 1) mbar_arrive(bar_sempty(slot / kGroup));
+          for (int i = 0; i < 16; i += 2) fma_pair(acc[q + i], acc[q + i + 1], p[h][i], p[h][i + 1], s2);
+          if (q + 16 < kCols) tmem_wait_ld();
+          if (q + 32 == kCols) {  // the buffer has been read
+            tc_fence_before();
+            __syncwarp();
+            mbar_arrive_if<PAIR>(tempty_at + 8u * buf, lane == 0);
+            mbar_arrive_if<false>(bar_sempty(slot / kGroup), lane == 0 && step % kGroup == kGroup - 1);
+          }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
+      int m, n;
+      tile_at<kRows>(a, t, m, n);
+      const int row0 = m * kRows + rank * kBM + (warp & 3) * 32, col0 = n * kBN + group * kCols;
       const int64_t row = row0 + lane;
       const bool live = ok && row < a.M && col0 < a.N;
+      const uint32_t stage = base + L::kOutOff + warp * kWarpOut;
       if (a.bias) {
+        const float* bias = reinterpret_cast<const float*>(base_ptr + L::kBiasOff) + warp * kCols;
 #pragma unroll
         for (int i = 0; i < kCols; i += 4) {
           const float4 v = *reinterpret_cast<const float4*>(bias + i);
@@ -344,28 +465,20 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       }
       if (a.act == XDIT_ACT_GELU_TANH) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) acc[i] = gelu_tanh(acc[i]);
+        for (int i = 0; i < kCols; i += 2) gelu_tanh2(acc[i], acc[i + 1]);
       }
       if (a.tma_out) {  // the last tile's results have left the staging buffer
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
       }
       if (a.out_q) {
-        // two warpgroups hold a block of 128 columns: they exchange their rows' largest magnitudes.  The buffer
-        // alternates, so the wait of one tile also keeps the next one's writes off it.
+        // the thread holds a whole block of its row; columns behind the end were loaded as zeros and are zeros still
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < kCols; ++i)
-          if (col0 + i < a.N) top = amax_nan(top, acc[i]);
-        float* buf = tops + (turn & 1) * 512;
-        buf[group * 128 + row_in] = top;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_top(group >> 1));
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_top(group >> 1), turn & 1, abort_flag, a.wait_limit_ns, 330));
-        top = amax_nan(top, buf[(group ^ 1) * 128 + row_in]);
+        for (int i = 0; i < kCols; ++i) top = amax_nan(top, acc[i]);
         float inv;
         const float sc = block_scale(top, inv);
-        if (live && !(group & 1)) a.out_scale[(col0 / kBlock) * a.out_scale_ld + row] = sc;
+        if (live) a.out_scale[(col0 / kBlock) * a.out_scale_ld + row] = sc;
 #pragma unroll
         for (int i = 0; i < kCols; i += 16) {
           uint4 w;
@@ -373,17 +486,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
           w.y = pack_e4m3(acc[i + 4] * inv, acc[i + 5] * inv, acc[i + 6] * inv, acc[i + 7] * inv);
           w.z = pack_e4m3(acc[i + 8] * inv, acc[i + 9] * inv, acc[i + 10] * inv, acc[i + 11] * inv);
           w.w = pack_e4m3(acc[i + 12] * inv, acc[i + 13] * inv, acc[i + 14] * inv, acc[i + 15] * inv);
-          st_shared16(stage + lane * 64 + (((i >> 4) ^ ((lane >> 1) & 3)) << 4), w);  // 64-byte swizzle
+          st_shared16(stage + lane * 128 + (((i >> 4) ^ (lane & 7)) << 4), w);  // 128-byte swizzle
         }
       } else if (a.tma_out) {
 #pragma unroll
-        for (int i = 0; i < kCols; i += 8) {
+        for (int i = 0; i < kCols; i += 8) {  // two boxes of 64 columns
           uint4 w;
           w.x = pack16(a.out_dtype, acc[i], acc[i + 1]);
           w.y = pack16(a.out_dtype, acc[i + 2], acc[i + 3]);
           w.z = pack16(a.out_dtype, acc[i + 4], acc[i + 5]);
           w.w = pack16(a.out_dtype, acc[i + 6], acc[i + 7]);
-          st_shared16(stage + lane * 128 + (((i >> 3) ^ (lane & 7)) << 4), w);  // 128-byte swizzle
+          st_shared16(stage + (i >> 6) * 4096 + lane * 128 + ((((i & 63) >> 3) ^ (lane & 7)) << 4), w);  // 128-byte swizzle
         }
       } else if (live) {
         const int64_t o = row * a.out_srow + col0;
@@ -401,8 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       if (a.tma_out) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0 && ok && row0 < a.M && col0 < a.N) {  // what lies behind the end of a row or column is not written
-          tma_store_2d(&a.tm_out, stage, col0, row0);
+        if (lane == 0 && ok && row0 < a.M) {  // what lies behind the end of a row or column is not written
+          if (col0 < a.N) tma_store_2d(&a.tm_out, stage, col0, row0);
+          if (!a.out_q && col0 + 64 < a.N) tma_store_2d(&a.tm_out, stage + 4096, col0 + 64, row0);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
@@ -413,9 +527,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
   // ---------------- teardown ----------------
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if constexpr (PAIR) cluster_sync();  // neither leaves while the other may still reach its barriers or TMEM
+  if (warp == 8) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
   }
   report(a, abort_flag);
 }
@@ -445,11 +561,6 @@ template <int NB> struct RowsLayout {
   static_assert(kStages * kStageBytes >= 128 * NB * 4, "the ring holds the sums that a cluster exchanges");
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float4 load_cluster(uint32_t addr, uint32_t rank) {
   float4 v;
   asm volatile(
@@ -664,9 +775,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
   if (warp < 4) {
     const float bias = a.bias && n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
+    for (int i = 0; i < NB; i += 2) {
       y[i] += bias;
-      if (a.act == XDIT_ACT_GELU_TANH) y[i] = gelu_tanh(y[i]);
+      y[i + 1] += bias;
+      if (a.act == XDIT_ACT_GELU_TANH) gelu_tanh2(y[i], y[i + 1]);
     }
   }
   if (a.out_q && !skip) {
@@ -838,20 +950,44 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
     if (p->M <= 32) return launch_rows<32>(a, *p, sms, quantise, (cudaStream_t)stream);
     return launch_rows<64>(a, *p, sms, quantise, (cudaStream_t)stream);
   }
+  // Pairs of CTAs take tiles of 256 rows, single CTAs of 128.  A pair reads W once for twice the rows, but starts and
+  // ends later and wastes more of a last, partly filled wave: it is worth it from four waves on (5120 x 5120: 2048
+  // rows 58 us by pairs and 56 by single CTAs, 4096 rows 98 and 103, 18,900 rows 409 and 437).
+  const int mt2 = (p->M + 2 * kBM - 1) / (2 * kBM);
+  const bool pairs = (int64_t)a.mt * a.nt > 3 * sms;
+  if (pairs) a.mt = mt2;
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
   if ((rc = encode_map(&a.tm_x, u8, 1, p->x, p->M, p->K, p->x_stride_row, kBM, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-  if ((rc = encode_map(&a.tm_w, u8, 1, p->w, p->N, p->K, p->w_stride_row, kBN, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+  if ((rc = encode_map(&a.tm_w, u8, 1, p->w, p->N, p->K, p->w_stride_row, pairs ? kBN / 2 : kBN, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   a.tma_out = p->out_q || (a.wide && es == 2);
   if (p->out_q)
-    rc = encode_map(&a.tm_out, u8, 1, p->out_q, p->M, p->N, p->N, 32, kCols, CU_TENSOR_MAP_SWIZZLE_64B);
+    rc = encode_map(&a.tm_out, u8, 1, p->out_q, p->M, p->N, p->N, 32, kCols, CU_TENSOR_MAP_SWIZZLE_128B);
   else if (a.tma_out)
-    rc = encode_map(&a.tm_out, u16, 2, p->out, p->M, p->N, p->out_stride_row, 32, kCols, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = encode_map(&a.tm_out, u16, 2, p->out, p->M, p->N, p->out_stride_row, 32, 64, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   const int64_t tiles = (int64_t)a.mt * a.nt;
   if (tiles > 0x3fffffffll) { set_error("%s: too many tiles", who); return XDIT_E_SHAPE; }
-  if ((rc = configure_smem<fp8_gemm_kernel>(kSmem))) return rc;
-  fp8_gemm_kernel<<<(int)(tiles < sms ? tiles : sms), kThreads, kSmem, (cudaStream_t)stream>>>(a);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (pairs) {
+    if ((rc = configure_smem<fp8_gemm_kernel<true>>(GemmLayout<true>::kSmem))) return rc;
+    const int most = sms / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * (tiles < most ? tiles : most)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = GemmLayout<true>::kSmem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<true>, a);
+  } else {
+    if ((rc = configure_smem<fp8_gemm_kernel<false>>(GemmLayout<false>::kSmem))) return rc;
+    fp8_gemm_kernel<false><<<(int)(tiles < sms ? tiles : sms), kThreads, GemmLayout<false>::kSmem, (cudaStream_t)stream>>>(a);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_kernel launch");
   return XDIT_OK;
 }
