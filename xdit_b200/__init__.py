@@ -7,6 +7,10 @@ Public surface (same names as the reference modules they stand in for):
 * ``xdit_b200.attention_backend``   -- ``AttentionBackendType``, ``ATTENTION_FUNCTION_REGISTRY``, ``register_attention_function``
 * ``xdit_b200.cache_manager``       -- ``get_cache_manager`` (PipeFusion stale-KV buffers)
 * ``xdit_b200.distributed``         -- sequence-parallel groups and the runtime state the path reads
+* ``xdit_b200.prologue``            -- the attention from a layer's projections, or from its hidden states
+* ``xdit_b200.rotary``              -- ``RotaryEmbedding``, ``rotary_embed``: rotary positions with several axes
+* ``xdit_b200.modulation``          -- ``gated_residual_norm``: gated residual and modulated norm between two sub-layers
+* ``xdit_b200.fp8_linear``          -- ``fp8_linear``, ``quantize_rows``, ``quantize_weight``: linear layers in 8-bit floating point
 * ``xdit_b200.ops``                 -- tensor-level wrappers over the C ABI declared in ``include/xdit_b200.h``
 
 All arithmetic runs in ``libxdit_b200.so`` (built in-tree by ``python -m xdit_b200.build``).

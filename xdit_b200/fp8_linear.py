@@ -71,6 +71,11 @@ def fp8_linear(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optiona
         out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
         lead, data, scale = x.shape[:-1], x.data, x.scale
         M = data.shape[0]
+    if torch.compiler.is_compiling():
+        from . import compile_ops
+
+        made = compile_ops.fp8_linear(data, scale, w, ws, bias, activation or "", out_dtype, quantize_out)
+        return Fp8Rows(made[0], made[1], tuple(lead)) if quantize_out else made[0].view(*lead, w.shape[0])
     if quantize_out:
         q, s = ops.empty_fp8_rows(M, w.shape[0], data.device)
         ops.fp8_linear(data, scale, w, ws, bias, activation=activation, out_q=q, out_scale=s)

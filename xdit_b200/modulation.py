@@ -35,6 +35,14 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] =
     projection that follows (C a multiple of 16)."""
     if residual.dim() != 3:
         raise ValueError("expected [B, s, C]")
+    if torch.compiler.is_compiling() and out_residual is None:
+        from . import compile_ops
+
+        made = list(compile_ops.gated_residual_norm(residual, branch, gate, float(residual_scale), post_norm or "",
+                                                    post_weight, post_bias, norm or "", weight, bias, scale, shift,
+                                                    float(eps), quantize))
+        hidden = made.pop(0) if branch is not None else residual
+        return hidden, Fp8Rows(*made, tuple(residual.shape[:2])) if quantize else made[0] if made else None
     if quantize and (norm is None or residual.shape[2] % 16):
         raise ValueError("quantize needs a norm and rows of a multiple of 16 values")
     if branch is None and out_residual is not None:

@@ -14,7 +14,9 @@ It stands for these lines of the reference's processors::
 (the same steps with a per-head norm in ``transformer_flux.py:113-147,170-219``).  The norm modules
 and Flux's rotary helper come from diffusers, which the reference does not vendor: the norm is
 ``torch.nn.RMSNorm`` semantics, the rotary embedding is the interleaved-pair form that the Wan
-processor defines inline.
+processor defines inline.  In place of cos/sin tables every function here takes a
+:class:`~xdit_b200.rotary.RotaryEmbedding`, and :func:`attention_from_hidden_states` starts and ends one step further out, with
+projections in 8-bit floating point.
 """
 from __future__ import annotations
 
@@ -27,7 +29,8 @@ from . import ops
 from . import usp as _usp
 from .distributed import (PROCESS_GROUP, get_ring_parallel_world_size, get_ulysses_parallel_rank,
                           get_ulysses_parallel_world_size)
-from .rotary import RotaryEmbedding
+from .fp8_linear import Fp8Rows, Fp8Weight, fp8_linear
+from .rotary import RotaryEmbedding, rotary_embed
 
 
 def qk_norm_rope_heads(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, heads: int, *,
@@ -40,20 +43,32 @@ def qk_norm_rope_heads(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     ``[heads, B, s, D]`` buffers viewed with the batch axis first."""
     B, s, HD = query.shape
     D = HD // heads
-    cos, sin = _cos_sin(rotary_emb, s, D, query.device)
+    cos, sin, late = _rotary(rotary_emb, B, s, D, query.device)
     n = heads * B * s * D
     buf = torch.empty(3 * n, dtype=query.dtype, device=query.device)
     ops.qk_norm_rope_pack(query, key, value, heads, buf, buf[n:], buf[2 * n:], (n, n, n), 1,
                           norm_q_weight=norm_q_weight, norm_k_weight=norm_k_weight, eps=eps,
                           norm_per_head=norm_per_head, cos=cos, sin=sin)
-    return tuple(buf[i * n:(i + 1) * n].view(heads, B, s, D).permute(1, 0, 2, 3) for i in range(3))
+    q, k, v = (buf[i * n:(i + 1) * n].view(heads, B, s, D).permute(1, 0, 2, 3) for i in range(3))
+    if late is not None:
+        rotary_embed(q, k, late, out_query=q, out_key=k)
+    return q, k, v
 
 
-def _cos_sin(rotary_emb, s, D, device):
+def _rotary(rotary_emb, B, s, D, device):
+    """``(cos, sin, late)``: the tables of the prologue kernel, which rotates interleaved pairs by one set of positions for
+    all samples, or the embedding that is applied behind it (halves, positions of each sample's own)."""
+    if isinstance(rotary_emb, RotaryEmbedding):
+        p = rotary_emb.positions
+        if rotary_emb.pairing != "interleaved" or (B > 1 and p is not None and p.dim() == 3 and p.shape[0] > 1):
+            return None, None, rotary_emb
+        return (*rotary_emb.tables(s, D, device), None)
+    return (*_cos_sin(rotary_emb, s, D), None)
+
+
+def _cos_sin(rotary_emb, s, D):
     if rotary_emb is None:
         return None, None
-    if isinstance(rotary_emb, RotaryEmbedding):
-        return rotary_emb.tables(s, D, device)
     cos, sin = rotary_emb
     # the processors carry [1, s, 1, D] tables (transformer_wan.py:108-120); [s, D] is accepted as well
     cos = cos.reshape(s, D) if cos.numel() == s * D else cos
@@ -69,14 +84,14 @@ def attention_from_projections(query: torch.Tensor, key: torch.Tensor, value: to
                                norm_per_head: bool = False,
                                rotary_emb: Union[RotaryEmbedding, Tuple[torch.Tensor, torch.Tensor], None] = None,
                                softmax_scale: Optional[float] = None,
-                               out_proj_weight: Optional[torch.Tensor] = None,
+                               out_proj_weight: Union[torch.Tensor, Fp8Weight, None] = None,
                                out_proj_bias: Optional[torch.Tensor] = None, attn_layer=None) -> torch.Tensor:
     """Self-attention of one DiT layer from its q/k/v projections ``[B, s_local, heads*D]`` to the
     tensor the output projection takes, ``[B, s_local, heads*D]``, under the current sequence-parallel
     degrees.  With a Ulysses degree ``U > 1`` and no ring the prologue kernel writes straight into the
     all-to-all send buffer; otherwise it produces ``[B, heads, s, D]`` tensors for ``USP``'s data path.
 
-    With ``out_proj_weight`` (``[hidden, heads*D]``, optional bias) the layer's output projection
+    With ``out_proj_weight`` (``[hidden, heads*D]`` or an ``Fp8Weight`` of it, optional bias) the layer's output projection
     (``attn.to_out[0]``, ``transformer_wan.py:152``, ``transformer_flux.py:210-219``) is applied as well and
     ``[B, s_local, hidden]`` is returned: the attention kernel writes its rows head-merged, so the
     projection reads them where they lie.
@@ -88,14 +103,41 @@ def attention_from_projections(query: torch.Tensor, key: torch.Tensor, value: to
     if attn_layer is not None:
         out = _attention_with_stale_kv(query, key, value, heads, norm_q_weight, norm_k_weight, eps, norm_per_head,
                                        rotary_emb, softmax_scale, attn_layer)
-        if out_proj_weight is not None:
-            out = torch.nn.functional.linear(out, out_proj_weight, out_proj_bias)
-        return out
+        return _project(out, out_proj_weight, out_proj_bias)
     out = _attention_from_projections(query, key, value, heads, norm_q_weight, norm_k_weight, eps, norm_per_head,
                                       rotary_emb, softmax_scale)
-    if out_proj_weight is not None:
-        out = torch.nn.functional.linear(out, out_proj_weight, out_proj_bias)
-    return out
+    return _project(out, out_proj_weight, out_proj_bias)
+
+
+def _project(x, weight, bias, out_dtype=None):
+    if weight is None:
+        return x
+    if isinstance(weight, Fp8Weight):
+        return fp8_linear(x, weight, bias, out_dtype=out_dtype)
+    return torch.nn.functional.linear(x, weight, bias)
+
+
+def attention_from_hidden_states(hidden_states: Union[torch.Tensor, Fp8Rows], qkv_weight: Union[torch.Tensor, Fp8Weight],
+                                 heads: int, *, qkv_bias: Optional[torch.Tensor] = None,
+                                 out_proj_weight: Union[torch.Tensor, Fp8Weight, None] = None,
+                                 out_proj_bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
+                                 **kwargs) -> torch.Tensor:
+    """Self-attention of one DiT layer from its (normed) hidden states ``[B, s_local, hidden]``: the fused q, k, v projection
+    ``qkv_weight`` ``[3 * heads*D, hidden]``, :func:`attention_from_projections` with ``kwargs`` on its three column slices, and the
+    output projection where one is given.  A weight may be an :class:`~xdit_b200.fp8_linear.Fp8Weight`; ``hidden_states`` may then
+    be the :class:`~xdit_b200.fp8_linear.Fp8Rows` that ``gated_residual_norm(quantize=True)`` makes, and ``dtype`` is the type that
+    the attention runs in."""
+    if isinstance(hidden_states, Fp8Rows):
+        if not isinstance(qkv_weight, Fp8Weight):
+            raise TypeError("e4m3 hidden states need an Fp8Weight as qkv_weight")
+    else:
+        dtype = hidden_states.dtype
+    qkv = _project(hidden_states, qkv_weight, qkv_bias, dtype)
+    if qkv.dim() != 3 or qkv.shape[2] % (3 * heads):
+        raise ValueError(f"expected [B, s, hidden] and a weight of 3 x {heads} heads, got a projection {tuple(qkv.shape)}")
+    query, key, value = qkv.chunk(3, dim=2)
+    return attention_from_projections(query, key, value, heads, out_proj_weight=out_proj_weight,
+                                      out_proj_bias=out_proj_bias, **kwargs)
 
 
 def _attention_with_stale_kv(query, key, value, heads, norm_q_weight, norm_k_weight, eps, norm_per_head, rotary_emb,
@@ -109,7 +151,7 @@ def _attention_with_stale_kv(query, key, value, heads, norm_q_weight, norm_k_wei
     D = HD // heads
     kc, vc, start = get_cache_manager().rows_for_producer(attn_layer, B, heads, n, D, query.dtype, query.device)
     S = kc.shape[2]
-    cos, sin = _cos_sin(rotary_emb, n, D, query.device)
+    cos, sin, late = _rotary(rotary_emb, B, n, D, query.device)
     q_buf = torch.empty(heads * B * n * D, dtype=query.dtype, device=query.device)
     # q in the packed [H][B][n][D] layout; k and v rows at [start, start + n) of the [B,H,S,D] buffers
     ops.qk_norm_rope_pack(query, key, value, heads, q_buf, kc.view(-1)[start * D:], vc.view(-1)[start * D:],
@@ -117,6 +159,9 @@ def _attention_with_stale_kv(query, key, value, heads, norm_q_weight, norm_k_wei
                           norm_per_head=norm_per_head, cos=cos, sin=sin,
                           dst_strides=[None, (S * D, heads * S * D), (S * D, heads * S * D)])
     q4 = q_buf.view(heads, B, n, D).permute(1, 0, 2, 3)
+    if late is not None:
+        k_new = kc[:, :, start:start + n]
+        rotary_embed(q4, k_new, late, out_query=q4, out_key=k_new)
     out = torch.empty(B, n, heads, D, dtype=query.dtype, device=query.device)
     ops.attn_fwd(q4, kc, vc, out=out.permute(0, 2, 1, 3), scale=softmax_scale)
     return out.view(B, n, HD)
@@ -148,13 +193,16 @@ def _attention_from_projections(query, key, value, heads, norm_q_weight, norm_k_
         return out.permute(0, 2, 1, 3).reshape(B, s, HD)
     assert heads % U == 0, "h must be divisible by world_size, got {} and {}".format(heads, U)
     Hl = heads // U
-    cos, sin = _cos_sin(rotary_emb, s, D, query.device)
+    cos, sin, late = _rotary(rotary_emb, B, s, D, query.device)
     blk = Hl * B * s * D
     stride = 3 * blk
     send = torch.empty(U * stride, dtype=query.dtype, device=query.device)
     ops.qk_norm_rope_pack(query, key, value, heads, send, send[blk:], send[2 * blk:], (stride, stride, stride), U,
                           norm_q_weight=norm_q_weight, norm_k_weight=norm_k_weight, eps=eps,
                           norm_per_head=norm_per_head, cos=cos, sin=sin)
+    for peer in range(U if late is not None else 0):
+        q, k = (send.as_strided((B, Hl, s, D), (s * D, B * s * D, D, 1), peer * stride + i * blk) for i in range(2))
+        rotary_embed(q, k, late, out_query=q, out_key=k)
     recv = torch.empty_like(send)
     dist.all_to_all_single(recv, send, group=PROCESS_GROUP.ULYSSES_PG)
     shape, strides = (B, Hl, U, s, D), (s * D, B * s * D, stride, D, 1)

@@ -90,6 +90,14 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], embedding: Ro
     fewer) in bf16, fp16 or fp32, any strides with a contiguous last axis.  The results lie in memory like the inputs, or
     go to ``out_query`` / ``out_key``, which may be the inputs themselves.  Angles are taken in 64 bits and their cos and
     sin in 32; a result is rounded once."""
+    if torch.compiler.is_compiling() and out_query is None and out_key is None:
+        from . import compile_ops
+
+        e = embedding
+        got = compile_ops.rotary_axes(query, key, e.positions, list(e.axes_dim), None if e.grid is None else list(e.grid),
+                                      e.start, e.theta, e.ladder, None if e.frequencies is None else list(e.frequencies),
+                                      e.pairing)
+        return got[0], got[1] if key is not None else None
     if query.dim() != 4 or (key is not None and key.dim() != 4):
         raise ValueError("query and key must be [B, heads, s, D]")
     if key is None and out_key is not None:
