@@ -444,6 +444,7 @@ struct xdit_fp8_linear_params {
   int32_t raw_dtype, raw_s;
   const void* raw;
   int64_t raw_stride_b, raw_stride_row;
+  int32_t selftest_stall; /* test aid: != 0 leaves the operands unloaded, so that the kernel's waits run out */
 };
 XDIT_API int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* stream);
 

@@ -250,3 +250,21 @@ def test_a_pending_failure_is_reported_and_cleared():
         fp8_linear(x, w)
     assert e.value.code == -6
     _check(x, w)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 384, 1024), (40, 5120, 5120), (200, 512, 384), (8000, 4096, 256)])
+def test_a_wait_that_runs_out_is_reported_by_the_next_call(M, N, K):
+    """Nothing is loaded, so the kernel's waits run out after a millisecond; it drains, sets the status words and ends, the next
+    call raises and launches nothing, and the one after it runs again.  Few rows (with and without a split of K), tiles of
+    single CTAs and of pairs."""
+    from xdit_b200._capi import XditError
+
+    x, w = _rows(M, K, 30), _weight(N, K, 31)
+    out = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ops.fp8_linear(x.data, x.scale, w.data, w.scale, out=out, _wait_limit_ns=1_000_000, _selftest_stall=True)
+    torch.cuda.synchronize()
+    assert torch.isnan(out).all()
+    with pytest.raises(XditError) as e:
+        ops.fp8_linear(x.data, x.scale, w.data, w.scale, out=out)
+    assert e.value.code == -6
+    _check(x, w)

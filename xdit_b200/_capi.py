@@ -185,7 +185,7 @@ class Fp8LinearParams(C.Structure):
         ("out_q", C.c_void_p), ("out_scale", C.c_void_p), ("out_scale_ld", C.c_int64),
         ("status", C.c_void_p), ("status_host", C.c_void_p), ("wait_limit_ns", C.c_uint32),
         ("raw_dtype", C.c_int32), ("raw_s", C.c_int32), ("raw", C.c_void_p),
-        ("raw_stride_b", C.c_int64), ("raw_stride_row", C.c_int64),
+        ("raw_stride_b", C.c_int64), ("raw_stride_row", C.c_int64), ("selftest_stall", C.c_int32),
     ]
 
 

@@ -82,6 +82,7 @@ struct alignas(64) GemmArgs {
   int32_t* status;
   int32_t* status_host;
   uint32_t wait_limit_ns;
+  int32_t selftest_stall;  // test aid: nothing is loaded, so the first waits run out
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       // ======================= TMA producer =======================
       if (lane == 0) {
         int issued = 0;
-        bool ok = true;
+        bool ok = a.selftest_stall == 0;
         for (int t = tile0; t < tiles && ok; t += tile_step) {
           int m, n;
           tile_at<kRows>(a, t, m, n);
@@ -311,6 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         }
         if (!ok) {
           // drain: every armed stage must have received its bytes before the CTA may leave (a pair: before either leaves)
+          // (the second CTA's bytes count on the first one's barriers, which it cannot watch: it leaves them a thousand times
+          // the time that a load takes)
+          if (rank) for (int it = 0; it < (1 << 14); ++it) __nanosleep(128);
           for (int i = rank ? issued : issued > kStages ? issued - kStages : 0; i < issued; ++i)
             for (int it = 0; it < (1 << 20) && !mbar_try_wait(bar_full(i % kStages), (i / kStages) & 1); ++it) __nanosleep(64);
         }
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         // the thread holds a whole block of its row; columns behind the end were loaded as zeros and are zeros still
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) top = amax_nan(top, acc[i]);
+        for (int i = 0; i < kCols; i += 2) top = amax_nan(top, acc[i], acc[i + 1]);
         float inv;
         const float sc = block_scale(top, inv);
         if (live) a.out_scale[(col0 / kBlock) * a.out_scale_ld + row] = sc;
@@ -546,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 // The kernel may start while the one that quantises x is still running (griddepcontrol): W is loaded at once, x and
 // its scales after that kernel's end.
 constexpr int kRowsThreads = 224;
+constexpr int kMaxSplits = 8;  // the largest portable cluster
 
 template <int NB> struct RowsLayout {
   static constexpr int kStages = NB <= 16 ? 6 : NB <= 32 ? 5 : 4;
@@ -627,12 +632,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
       auto load_x = [&](int i) {
         tma_load_2d(base + (i % kStages) * L::kStageBytes + kABytes, &a.tm_x, bar_full(i % kStages), (c0 + i) * kBK, m0);
       };
-      const int first = min(steps, kStages);
+      const int first = a.selftest_stall ? 0 : min(steps, kStages);
       for (int i = 0; i < first; ++i) load_w(i);
       asm volatile("griddepcontrol.wait;" ::: "memory");  // x is complete from here on
       for (int i = 0; i < first; ++i) load_x(i);
       int issued = first;
-      for (; issued < steps; ++issued) {
+      ok = a.selftest_stall == 0;
+      for (; ok && issued < steps; ++issued) {
         ok = mbar_wait(bar_empty(issued % kStages), (issued / kStages - 1) & 1, abort_flag, a.wait_limit_ns, 100);
         if (!ok) break;
         load_w(issued);
@@ -714,18 +720,21 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
       __syncwarp();
       tc_fence_after();
       const float* scales = reinterpret_cast<const float*>(base_ptr + L::kScaleOff + slot * L::kSlot);
-      const float sw = scales[NB];
+      const uint64_t sw = f2_pack(scales[NB], scales[NB]);
+      uint32_t p[2][16];
+      XDIT_TMEM_LD16(p[0], taddr + buf * NB);
+      tmem_wait_ld();
 #pragma unroll
       for (int q = 0; q < NB; q += 16) {
-        uint32_t p[16];
-        XDIT_TMEM_LD16(p, taddr + buf * NB + q);
-        tmem_wait_ld();
+        const int h = (q >> 4) & 1;
+        if (q + 16 < NB) XDIT_TMEM_LD16(p[h ^ 1], taddr + buf * NB + q + 16);  // while these are added
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const float4 sx = *reinterpret_cast<const float4*>(scales + q + i);
-          fma_pair(acc[q + i], acc[q + i + 1], p[i], p[i + 1], f2_pack(sx.x * sw, sx.y * sw));
-          fma_pair(acc[q + i + 2], acc[q + i + 3], p[i + 2], p[i + 3], f2_pack(sx.z * sw, sx.w * sw));
+          fma_pair(acc[q + i], acc[q + i + 1], p[h][i], p[h][i + 1], f2_mul(f2_pack(sx.x, sx.y), sw));
+          fma_pair(acc[q + i + 2], acc[q + i + 3], p[h][i + 2], p[h][i + 3], f2_mul(f2_pack(sx.z, sx.w), sw));
         }
+        if (q + 16 < NB) tmem_wait_ld();
       }
       tc_fence_before();
       __syncwarp();
@@ -738,76 +747,84 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
   }
 
   // ======================= epilogue =======================
-  // Rows [first, last) of the tile of x are this CTA's; without a split they are all of them.
-  const int share = NB / a.splits, first = split * share, last = first + share;
-  if (a.splits > 1) {
-    // every MMA of this CTA has read the ring by now: the summing warps have waited for all of them
-    if (warp < 4) {
-      float* mine = reinterpret_cast<float*>(base_ptr);  // [128 rows of W][NB], rotated so that neighbours use other banks
-#pragma unroll
-      for (int i = 0; i < NB; i += 4)
-        *reinterpret_cast<float4*>(mine + (warp * 32 + lane) * NB + ((i + 4 * lane) & (NB - 1))) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-    }
-    cluster_sync();
-  }
-  float y[NB];
+  // The sums go to shared memory, [128 rows of W][NB], where the ring was: every MMA has read it by now, for the summing
+  // warps have waited for all of them.  Rows [first, last) of the tile of x are this CTA's (without a split all of them):
+  // it adds the cluster's sums of these, and nobody else reads its own ones, which take the results.  (Short loops, not
+  // unrolled ones on the registers: with 64 rows the code that runs once cost 3 us more.)
+  const int share = NB / a.splits, first = split * share, last = min(first + share, a.M - m0);
+  const int n = n0 + warp * 32 + lane;
+  const uint32_t mine = base + (warp * 32 + lane) * (NB * 4);
+  auto place = [&](int i) { return (uint32_t)((i + 4 * lane) & (NB - 1)) * 4; };  // rotated: neighbours use other banks
   if (warp < 4) {
-    if (a.splits > 1) {
 #pragma unroll
-      for (int i = 0; i < NB; i += 4) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i + 4 > first && i < last) {
-          const uint32_t at = base + ((warp * 32 + lane) * NB + ((i + 4 * lane) & (NB - 1))) * 4;
-          for (int c = 0; c < a.splits; ++c) {
-            const float4 u = load_cluster(at, c);
-            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    for (int i = 0; i < NB; i += 4)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + place(i)), "f"(acc[i]), "f"(acc[i + 1]), "f"(acc[i + 2]), "f"(acc[i + 3]) : "memory");
+  }
+  if (a.splits > 1) cluster_sync();
+  float* tops = reinterpret_cast<float*>(base_ptr + L::kTopOff);
+  if (warp < 4) {
+    const float bias = a.bias && n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f;
+    const int es = a.out_dtype == XDIT_F32 ? 4 : 2;
+    const int64_t row_bytes = a.out_srow * es;
+    char* o = reinterpret_cast<char*>(a.out) + (m0 + (first & ~3)) * row_bytes + (int64_t)n * es;
+    const bool write = ok && n < a.N;
+#pragma unroll 1
+    for (int i = first & ~3; i < last; i += 4) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 u[kMaxSplits];  // all on their way before the first is added: a load from another SM takes long
+#pragma unroll
+      for (int c = 0; c < kMaxSplits; ++c)
+        if (c < a.splits) u[c] = a.splits > 1 ? load_cluster(mine + place(i), c) : *reinterpret_cast<const float4*>(base_ptr + (mine - base) + place(i));
+#pragma unroll
+      for (int c = 0; c < kMaxSplits; ++c)
+        if (c < a.splits) { v.x += u[c].x; v.y += u[c].y; v.z += u[c].z; v.w += u[c].w; }
+      float y[4] = {v.x + bias, v.y + bias, v.z + bias, v.w + bias};
+      if (a.act == XDIT_ACT_GELU_TANH) { gelu_tanh2(y[0], y[1]); gelu_tanh2(y[2], y[3]); }
+      if (a.out_q) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // a NaN's bits are above an infinity's
+          const uint32_t top = __reduce_max_sync(0xffffffffu, n < a.N ? __float_as_uint(fabsf(y[j])) : 0u);
+          if (lane == 0) tops[warp * NB + i + j] = __uint_as_float(top);
+        }
+        // rows of another CTA's share are left alone: it may be reading them
+        if (i >= first && i + 4 <= first + share) {
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + place(i)), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]) : "memory");
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (i + j >= first && i + j < last)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + place(i) + 4 * j), "f"(y[j]) : "memory");
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j, o += row_bytes) {
+          if (!write || i + j < first || i + j >= last) continue;
+          if (es == 4) {
+            *reinterpret_cast<float*>(o) = y[j];
+          } else {
+            const uint32_t w = pack16(a.out_dtype, y[j], 0.f);
+            *reinterpret_cast<uint16_t*>(o) = (uint16_t)w;
           }
         }
-        y[i] = v.x; y[i + 1] = v.y; y[i + 2] = v.z; y[i + 3] = v.w;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) y[i] = acc[i];
     }
   }
   if (a.splits > 1) cluster_sync();  // nobody leaves while its sums are being read
-  const int n = n0 + warp * 32 + lane;
-  if (warp < 4) {
-    const float bias = a.bias && n < a.N ? load_any(a.bias, a.bias_dtype, n) : 0.f;
-#pragma unroll
-    for (int i = 0; i < NB; i += 2) {
-      y[i] += bias;
-      y[i + 1] += bias;
-      if (a.act == XDIT_ACT_GELU_TANH) gelu_tanh2(y[i], y[i + 1]);
-    }
-  }
-  if (a.out_q && !skip) {
+  if (a.out_q) {
     // the tile's 128 columns of the result are one block: its rows' largest magnitudes over the four warps
-    float* tops = reinterpret_cast<float*>(base_ptr + L::kTopOff);
-    if (warp < 4) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, n < a.N ? __float_as_uint(fabsf(y[i])) : 0u);  // a NaN's bits are above an infinity's
-        if (lane == 0) tops[warp * NB + i] = __uint_as_float(top);
-      }
-    }
     __syncthreads();
     if (warp < 4 && ok) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int64_t m = m0 + i;
-        if (i < first || i >= last || m >= a.M) continue;
-        float inv;
-        const float top = amax_nan(amax_nan(tops[i], tops[NB + i]), amax_nan(tops[2 * NB + i], tops[3 * NB + i]));
+#pragma unroll 1
+      for (int i = first; i < last; ++i) {
+        float inv, y;
+        const float top = amax_nan(amax_nan(tops[i], tops[NB + i], tops[2 * NB + i]), tops[3 * NB + i]);
         const float sc = block_scale(top, inv);
-        if (n < a.N) a.out_q[m * a.N + n] = (uint8_t)pack_e4m3(y[i] * inv, 0.f, 0.f, 0.f);
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(mine + place(i & ~3) + 4 * (i & 3)) : "memory");
+        const int64_t m = m0 + i;
+        if (n < a.N) a.out_q[m * a.N + n] = (uint8_t)pack_e4m3(y * inv, 0.f, 0.f, 0.f);
         if (threadIdx.x == 0) a.out_scale[(n0 / kBlock) * a.out_scale_ld + m] = sc;
       }
     }
-  } else if (warp < 4 && ok && n < a.N) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-      if (i >= first && i < last && m0 + i < a.M) store_any(a.out, a.out_dtype, (int64_t)(m0 + i) * a.out_srow + n, y[i]);
   }
 
   // ---------------- teardown ----------------
@@ -866,7 +883,7 @@ int launch_rows(GemmArgs& a, const xdit_fp8_linear_params& p, int sms, bool afte
   if ((rc = encode_map(&a.tm_w, u8, 1, p.w, p.N, p.K, p.w_stride_row, 128, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   const int nt = (p.N + 127) / 128, mt = (p.M + NB - 1) / NB;
   a.splits = 1;
-  while (a.splits < 8 && (int64_t)nt * mt * a.splits * 2 <= 2 * sms && a.kb / (a.splits * 2) >= 4) a.splits *= 2;
+  while (a.splits < kMaxSplits && (int64_t)nt * mt * a.splits * 2 <= 2 * sms && a.kb / (a.splits * 2) >= 4) a.splits *= 2;
   if ((rc = configure_smem<fp8_rows_kernel<NB>>(L::kSmem))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(nt * a.splits), (unsigned)mt);
@@ -945,6 +962,7 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   a.wide = ((uintptr_t)p->out) % 16 == 0 && (p->M == 1 || (p->out_stride_row * es) % 16 == 0);
   a.status = p->status; a.status_host = p->status_host;
   a.wait_limit_ns = p->wait_limit_ns ? p->wait_limit_ns : kWaitLimitNs;
+  a.selftest_stall = p->selftest_stall;
   if (p->M <= 64) {
     if (p->M <= 16) return launch_rows<16>(a, *p, sms, quantise, (cudaStream_t)stream);
     if (p->M <= 32) return launch_rows<32>(a, *p, sms, quantise, (cudaStream_t)stream);

@@ -16,6 +16,12 @@ __device__ __forceinline__ float amax_nan(float m, float x) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
   return r;
 }
+// The largest of m and two absolute values (m is one already); a NaN wins.
+__device__ __forceinline__ float amax_nan(float m, float x, float y) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(x), "f"(y));
+  return r;
+}
 // Scale of a block whose largest magnitude is `top`, and its reciprocal (both powers of two).
 __device__ __forceinline__ float block_scale(float top, float& inverse) {
   const uint32_t bits = __float_as_uint(top);

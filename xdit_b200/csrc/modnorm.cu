@@ -328,16 +328,18 @@ gated_residual_norm_kernel(const __grid_constant__ NormArgs a) {
           for (int i = 0; i < 4; ++i) split(h[k][i], x[2 * i], x[2 * i + 1]);
           if (idx < a.nvec) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = amax_nan(top, x[i]);
+            for (int i = 0; i < 8; i += 2) top = amax_nan(top, x[i], x[i + 1]);
           }
 #pragma unroll
           for (int m = 8; m > 0; m >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
           float inv;
           const float sc = block_scale(top, inv);
           if (idx < a.nvec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split(mul(h[k][i], both<E>(inv)), x[2 * i], x[2 * i + 1]);
             uint2 q;
-            q.x = pack_e4m3(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-            q.y = pack_e4m3(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+            q.x = pack_e4m3(x[0], x[1], x[2], x[3]);
+            q.y = pack_e4m3(x[4], x[5], x[6], x[7]);
             *reinterpret_cast<uint2*>(a.out_q + (int64_t)r * a.C + idx * 8) = q;
             if (idx % 16 == 0) a.out_scale[(idx / 16) * a.scale_ld + r] = sc;
           }
@@ -378,7 +380,7 @@ quantize_rows_kernel(const T* x, int64_t sb, int64_t srow, int s, int64_t rows, 
           for (int j = 0; j < 4; ++j) split(p[j], v[2 * j], v[2 * j + 1]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = amax_nan(top, v[j]);
+        for (int j = 0; j < 8; j += 2) top = amax_nan(top, v[j], v[j + 1]);
 #pragma unroll
         for (int m = 8; m > 0; m >>= 1) top = amax_nan(top, __shfl_xor_sync(0xffffffffu, top, m));
         float inv;

@@ -821,7 +821,8 @@ _ACTIVATIONS = {None: _capi.XDIT_ACT_NONE, "gelu_tanh": _capi.XDIT_ACT_GELU_TANH
 def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor, w_scale: torch.Tensor,
                bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
                out: Optional[torch.Tensor] = None, out_q: Optional[torch.Tensor] = None,
-               out_scale: Optional[torch.Tensor] = None, _wait_limit_ns: int = 0) -> None:
+               out_scale: Optional[torch.Tensor] = None, _wait_limit_ns: int = 0,
+               _selftest_stall: bool = False) -> None:
     """``out = act(x w^T + bias)`` with a weight ``w`` [N, K] in e4m3 and fp32 scales ``w_scale`` [N/128, K/128] of any value and
     strides (``xdit_fp8_linear``).  ``x``: e4m3 rows [M, K] with ``x_scale`` [M, K/128]; or, with ``x_scale`` ``None``, a bf16, fp16
     or fp32 tensor [B, s, K] that is quantised first (M = B*s).  ``out`` [M, N] in bf16, fp16 or fp32, or ``out_q`` with
@@ -878,7 +879,7 @@ def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor
     p = _capi.Fp8LinearParams(M, N, K, _ACTIVATIONS[activation], out_dtype, b[1], address, w.data_ptr(), xs[0] if given else K,
                               ws0, scales.data_ptr() if given else address + (M * K + 15) // 16 * 16, w_scale.data_ptr(),
                               scale_row, scale_block, *w_scale.stride(), b[0], *o, st.dev.data_ptr(), st.host.data_ptr(),
-                              _wait_limit_ns, *raw)
+                              _wait_limit_ns, *raw, _selftest_stall)
     _launch_attn(_capi.load().xdit_fp8_linear, p, x, "xdit_fp8_linear")
     launch_count += 1 if given else 2
 
