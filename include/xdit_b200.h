@@ -346,7 +346,7 @@ XDIT_API int xdit_qk_norm_rope_pack(const struct xdit_prologue_params* p, void* 
  * frequencies and axis are HOST arrays of `pairs` entries, read during the call.
  * Replaces: the inline apply_rotary_emb and the position tables of the processors
  * (transformer_wan.py:106-122, the frequencies' chunk at :311-319). */
-#define XDIT_ROTARY_MAX_PAIRS 256
+#define XDIT_ROTARY_MAX_PAIRS 128
 #define XDIT_ROTARY_MAX_AXES 4
 enum xdit_position_kind { XDIT_POS_GRID = 0, XDIT_POS_I32 = 1, XDIT_POS_I64 = 2, XDIT_POS_F32 = 3 };
 struct xdit_rotary_positions {

@@ -199,6 +199,39 @@ def test_strides_of_rows_scales_and_result(M):
     assert torch.isnan(buf[mask]).all()
 
 
+@pytest.mark.parametrize("M,N,K,dtype,act,bias", [
+    (4000, 4161, 272, torch.float32, None, True), (4097, 4096, 1040, torch.float16, "gelu_tanh", True),
+    (3841, 4328, 144, torch.bfloat16, None, False), (60000, 257, 16, torch.bfloat16, "gelu_tanh", False)])
+def test_many_tiles(M, N, K, dtype, act, bias):
+    """Sizes that go to pairs of CTAs: last tiles of one row or column, an odd number of blocks, several tiles a CTA."""
+    b = torch.randn(N, device="cuda", generator=_gen(32)).to(dtype) if bias else None
+    _check(_rows(M, K, 33, columns=M % 2 == 0), _weight(N, K, 34), b, act, dtype)
+
+
+@pytest.mark.parametrize("M,N,K", [(4100, 4112, 400), (30000, 528, 128)])
+def test_many_tiles_as_e4m3_rows(M, N, K):
+    """The e4m3 result is the fp32 result quantised by the rule: the same sums, so the same bits."""
+    x, w, b = _rows(M, K, 35), _weight(N, K, 36), torch.randn(N, device="cuda", generator=_gen(37))
+    r = fp8_linear(x, w, b, activation="gelu_tanh", quantize_out=True)
+    want = quantize_rows(fp8_linear(x, w, b, activation="gelu_tanh", out_dtype=torch.float32))
+    assert torch.equal(r.scale, want.scale) and torch.equal(r.data.view(torch.uint8), want.data.view(torch.uint8))
+
+
+@pytest.mark.parametrize("M,N", [(150, 200), (20, 200), (9000, 2008)])
+def test_aligned_result_inside_a_larger_buffer(M, N):
+    """Rows on 16-byte boundaries leave in boxes of 64 columns: nothing beside the result is written."""
+    K = 256
+    x, w = _rows(M, K, 38), _weight(N, K, 39)
+    buf = torch.full((M + 2, N + 16), float("nan"), dtype=torch.bfloat16, device="cuda")
+    out = buf[1:-1, 8:8 + N]
+    ops.fp8_linear(x.data, x.scale, w.data, w.scale, out=out)
+    want, tol = _want(x, w, None, None)
+    assert ((out.double() - want).abs() <= tol + want.abs() * 2.0 ** -8 + 1e-30).all()
+    mask = torch.ones_like(buf, dtype=torch.bool)
+    mask[1:-1, 8:8 + N] = False
+    assert torch.isnan(buf[mask]).all()
+
+
 def test_no_rows_and_leading_axes():
     w = _weight(144, 256, 20)
     assert fp8_linear(torch.empty(2, 0, 256, device="cuda"), w).shape == (2, 0, 144)

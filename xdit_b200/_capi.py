@@ -18,7 +18,7 @@ XDIT_MAX_PACK_JOBS = 4
 XDIT_MAX_OUT_SEGMENTS = 16
 XDIT_PEER_HANDLE_BYTES = 64
 XDIT_POS_GRID, XDIT_POS_I32, XDIT_POS_I64, XDIT_POS_F32 = 0, 1, 2, 3
-XDIT_ROTARY_MAX_PAIRS, XDIT_ROTARY_MAX_AXES = 256, 4
+XDIT_ROTARY_MAX_PAIRS, XDIT_ROTARY_MAX_AXES = 128, 4
 XDIT_NORM_NONE, XDIT_NORM_LAYER, XDIT_NORM_RMS = 0, 1, 2
 XDIT_NORM_MAX_C = 16384
 XDIT_FP8_BLOCK = 128

@@ -582,7 +582,7 @@ def qk_norm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: 
 
 def _check_tensors(first: torch.Tensor, *others) -> None:
     """What every launch asks of its tensors: no gradient to record, CUDA memory, one device."""
-    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+    if torch.is_grad_enabled() and (first.requires_grad or [t for t in others if t is not None and t.requires_grad]):
         raise NotImplementedError("backward passes are not part of this inference path: call it under "
                                   "torch.no_grad(), or with tensors that do not require a gradient")
     if not first.is_cuda:
@@ -615,31 +615,32 @@ def _rows_contiguous(t: torch.Tensor, name: str) -> None:
 _POSITIONS = {torch.int32: _capi.XDIT_POS_I32, torch.int64: _capi.XDIT_POS_I64, torch.float32: _capi.XDIT_POS_F32}
 
 
-def rotary_positions(frequencies, axis, axes: int, *, positions: Optional[torch.Tensor] = None,
+def rotary_positions(frequencies, axis, pairs: int, axes: int, *, positions: Optional[torch.Tensor] = None,
                      grid: Optional[Sequence[int]] = None, start: int = 0, batch: int = 1,
                      rows: int = 0) -> _capi.RotaryPositions:
-    """Positions and angles as the rotary kernels take them.  ``frequencies`` and ``axis`` are ctypes arrays
-    (double, uint8) with one entry for each rotated pair.  ``positions``: int32, int64 or fp32, ``[rows, axes]`` or
+    """Positions and angles as the rotary kernels take them.  ``frequencies`` and ``axis``: ctypes pointers
+    (double, uint8) to one entry for each of the rotated ``pairs``.  ``positions``: int32, int64 or fp32, ``[rows, axes]`` or
     ``[batch or 1, rows, axes]``; or ``grid``, the sides of a grid that the token index ``start + row`` walks."""
-    p = _capi.RotaryPositions(axes=axes, pairs=len(frequencies), frequencies=frequencies, axis=axis)
     if (positions is None) == (grid is None):
         raise ValueError("give either positions or a grid")
     if grid is not None:
         if len(grid) != axes or not 1 <= axes <= _capi.XDIT_ROTARY_MAX_AXES:
             raise ValueError(f"a grid of {len(grid)} sides for {axes} axes (1..{_capi.XDIT_ROTARY_MAX_AXES})")
-        p.kind, p.start = _capi.XDIT_POS_GRID, int(start)
-        for i, side in enumerate(grid):
-            p.grid[i] = int(side)
-        return p
-    if positions.dtype not in _POSITIONS:
+        return _capi.RotaryPositions(_capi.XDIT_POS_GRID, axes, pairs, frequencies, axis, None, 0, 0, 0,
+                                     _GRID(*[int(side) for side in grid]), int(start))
+    kind = _POSITIONS.get(positions.dtype)
+    if kind is None:
         raise TypeError(f"positions must be int32, int64 or fp32, not {positions.dtype}")
-    t = positions if positions.dim() == 3 else positions.unsqueeze(0)
-    if t.dim() != 3 or t.shape[0] not in (1, batch) or t.shape[1] != rows or t.shape[2] != axes:
-        raise ValueError(f"positions {tuple(positions.shape)} for {batch} samples of {rows} tokens on {axes} axes")
-    p.kind, p.positions = _POSITIONS[t.dtype], t.data_ptr()
-    p.stride_b = t.stride(0) if t.shape[0] > 1 else 0
-    p.stride_row, p.stride_axis = t.stride(1), t.stride(2)
-    return p
+    shape, stride = positions.shape, positions.stride()
+    each = len(shape) == 3
+    if len(shape) not in (2, 3) or shape[-2] != rows or shape[-1] != axes or (each and shape[0] not in (1, batch)):
+        raise ValueError(f"positions {tuple(shape)} for {batch} samples of {rows} tokens on {axes} axes")
+    return _capi.RotaryPositions(kind, axes, pairs, frequencies, axis, positions.data_ptr(),
+                                 stride[0] if each and shape[0] > 1 else 0, stride[-2], stride[-1])
+
+
+_PAIR = C.c_int64 * 2
+_GRID = C.c_int64 * _capi.XDIT_ROTARY_MAX_AXES
 
 
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.RotaryPositions, halves: bool,
@@ -667,9 +668,8 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.Rot
     if D != 1 and (q1 != 1 or o1 != 1 or k1 != 1 or p1 != 1):
         raise ValueError("the last axis of q, k and their outputs must be contiguous")
     _check_tensors(q, k, out_q, out_k)
-    pair = C.c_int64 * 2
     p = _capi.RotaryParams(dtype, B, H, Hk, s, D, halves, positions, q.data_ptr(), k_ptr, out_q.data_ptr(), out_k_ptr,
-                           pair(qb, kb), pair(qh, kh), pair(qs, ks), pair(ob, pb), pair(oh, ph), pair(os_, ps))
+                           _PAIR(qb, kb), _PAIR(qh, kh), _PAIR(qs, ks), _PAIR(ob, pb), _PAIR(oh, ph), _PAIR(os_, ps))
     _launch(_capi.load().xdit_rotary_axes, q, "xdit_rotary_axes", C.byref(p))
     launch_count += 1
 

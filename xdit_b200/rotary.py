@@ -21,7 +21,8 @@ from . import _capi, ops
 
 @lru_cache(maxsize=64)
 def _pairs(axes_dim: Tuple[int, ...], theta: float, ladder: str, frequencies: Optional[Tuple[float, ...]]):
-    """ctypes arrays of every rotated pair's frequency (radians at position one) and axis."""
+    """``(frequencies, axis, pairs)``: ctypes pointers to every rotated pair's frequency (radians at position one) and
+    axis (they keep their arrays alive)."""
     if not 1 <= len(axes_dim) <= _capi.XDIT_ROTARY_MAX_AXES or any(d < 0 or d % 2 for d in axes_dim):
         raise ValueError(f"axes_dim {axes_dim}: 1 to {_capi.XDIT_ROTARY_MAX_AXES} even numbers of elements")
     n = sum(axes_dim) // 2
@@ -38,10 +39,10 @@ def _pairs(axes_dim: Tuple[int, ...], theta: float, ladder: str, frequencies: Op
         freq = [theta ** (-float(i) / n) for i in range(n)]
     else:
         raise ValueError(f"ladder {ladder!r}: 'axis' or 'shared'")
-    return (C.c_double * n)(*freq), (C.c_uint8 * n)(*axis)
+    return (C.cast((C.c_double * n)(*freq), C.POINTER(C.c_double)), C.cast((C.c_uint8 * n)(*axis), C.POINTER(C.c_uint8)), n)
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False)
 class RotaryEmbedding:
     """Where tokens are, and how far their pairs turn.
 
@@ -65,9 +66,9 @@ class RotaryEmbedding:
     def _params(self, batch: int, rows: int):
         if self.pairing not in ("interleaved", "halves"):
             raise ValueError(f"pairing {self.pairing!r}: 'interleaved' or 'halves'")
-        freq, axis = _pairs(tuple(self.axes_dim), float(self.theta), self.ladder,
-                            tuple(self.frequencies) if self.frequencies is not None else None)
-        return ops.rotary_positions(freq, axis, len(self.axes_dim), positions=self.positions, grid=self.grid,
+        f = self.frequencies
+        freq, axis, pairs = _pairs(tuple(self.axes_dim), self.theta, self.ladder, f if f is None else tuple(f))
+        return ops.rotary_positions(freq, axis, pairs, len(self.axes_dim), positions=self.positions, grid=self.grid,
                                     start=self.start, batch=batch, rows=rows)
 
     def tables(self, s: int, D: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
