@@ -46,7 +46,10 @@ constexpr int kGroup = 4, kGroups = kAhead / kGroup;  // steps whose scales shar
 constexpr int kABytes = kBM * kBK;
 constexpr int kWarpOut = 32 * kCols * 2;  // staging of a summing warp's results
 constexpr int kScaleBytes = 576;          // 128 scales of x + 2 of w, padded
-constexpr int kBand = 2048;               // rows of a band: the tiles of a band are walked column by column
+// Bytes of x in a band of row tiles, whose tiles are walked column by column: the band stays in L2 while W passes, and the
+// fewer bands, the seldomer W passes (75,600 x 5120 x 15360: 10 MB 5.88 ms, 21 MB 5.75, 42 MB 5.83, 84 MB 6.35; 9450 x 13824 x
+// 5120: 14 MB 663 us, 28 MB 648, 57 MB 658, 113 MB 686).
+constexpr int64_t kBandBytes = 24 << 20;
 
 template <bool PAIR> struct GemmLayout {
   static constexpr int kStages = PAIR ? 4 : 3;
@@ -65,6 +68,7 @@ struct alignas(64) GemmArgs {
   CUtensorMap tm_x, tm_w, tm_out;
   int32_t M, N, kb;        // kb: blocks along K
   int32_t mt, nt;          // tiles
+  int32_t band;            // row tiles of a band
   int32_t splits;          // CTAs of a cluster that share the K axis of a tile (few rows)
   const float* xs;
   int64_t xs_srow, xs_skb;
@@ -210,14 +214,12 @@ __device__ __forceinline__ void report(const GemmArgs& a, volatile int* abort_fl
     }
   }
 }
-// Tile t: its first row and column of tiles, `rows` rows of x a tile.
-template <int ROWS>
+// Tile t: its row and column of tiles.
 __device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& m, int& n) {
-  constexpr int kHigh = kBand / ROWS;
-  const int band = t / (kHigh * a.nt), rem = t - band * kHigh * a.nt;
-  const int high = min(kHigh, a.mt - band * kHigh);
+  const int band = t / (a.band * a.nt), rem = t - band * a.band * a.nt;
+  const int high = min(a.band, a.mt - band * a.band);
   n = rem / high;
-  m = band * kHigh + rem - n * high;
+  m = band * a.band + rem - n * high;
 }
 
 template <bool PAIR>
@@ -282,11 +284,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     if (warp == 9) {
       // ======================= TMA producer =======================
       if (lane == 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // a kernel that quantises x may still be running until here
         int issued = 0;
         bool ok = a.selftest_stall == 0;
         for (int t = tile0; t < tiles && ok; t += tile_step) {
           int m, n;
-          tile_at<kRows>(a, t, m, n);
+          tile_at(a, t, m, n);
           for (int c = 0; c < a.kb; ++c) {
             const int st = issued % kStages, turn = issued / kStages;
             if (turn > 0) ok = mbar_wait(bar_empty(st), (turn - 1) & 1, abort_flag, a.wait_limit_ns, 100 + st);
@@ -322,11 +325,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     } else if (warp == 10) {
       // ======================= scales: each lane the rows lane, lane + 32, ... of the tile =======================
       // A load from L2 takes longer than a step, so they are copied asynchronously, up to kAhead steps ahead.
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       int step = 0;
       bool ok = true;
       for (int t = tile0; t < tiles && ok; t += tile_step) {
         int m, n;
-        tile_at<kRows>(a, t, m, n);
+        tile_at(a, t, m, n);
         const float* src[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     for (int t = tile0; t < tiles && ok; t += tile_step) {
       if (a.bias) {
         int m, n;
-        tile_at<kRows>(a, t, m, n);
+        tile_at(a, t, m, n);
         const int col0 = n * kBN + group * kCols;
         float* bias = reinterpret_cast<float*>(base_ptr + L::kBiasOff) + warp * kCols;
         __syncwarp();
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       }
       ok = __all_sync(0xffffffffu, ok);
       int m, n;
-      tile_at<kRows>(a, t, m, n);
+      tile_at(a, t, m, n);
       const int row0 = m * kRows + rank * kBM + (warp & 3) * 32, col0 = n * kBN + group * kCols;
       const int64_t row = row0 + lane;
       const bool live = ok && row < a.M && col0 < a.N;
@@ -974,6 +978,8 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   const int mt2 = (p->M + 2 * kBM - 1) / (2 * kBM);
   const bool pairs = (int64_t)a.mt * a.nt > 3 * sms;
   if (pairs) a.mt = mt2;
+  const int64_t band = kBandBytes / ((int64_t)p->K * (pairs ? 2 * kBM : kBM));
+  a.band = (int)(band < 1 ? 1 : band > a.mt ? a.mt : band);
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u16 = CU_TENSOR_MAP_DATA_TYPE_UINT16;
   if ((rc = encode_map(&a.tm_x, u8, 1, p->x, p->M, p->K, p->x_stride_row, kBM, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   if ((rc = encode_map(&a.tm_w, u8, 1, p->w, p->N, p->K, p->w_stride_row, pairs ? kBN / 2 : kBN, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
@@ -985,27 +991,23 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
   if (rc) return rc;
   const int64_t tiles = (int64_t)a.mt * a.nt;
   if (tiles > 0x3fffffffll) { set_error("%s: too many tiles", who); return XDIT_E_SHAPE; }
-  cudaError_t e;
-  if (pairs) {
-    if ((rc = configure_smem<fp8_gemm_kernel<true>>(GemmLayout<true>::kSmem))) return rc;
-    const int most = sms / 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * (tiles < most ? tiles : most)));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = GemmLayout<true>::kSmem;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 2;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<true>, a);
-  } else {
-    if ((rc = configure_smem<fp8_gemm_kernel<false>>(GemmLayout<false>::kSmem))) return rc;
-    fp8_gemm_kernel<false><<<(int)(tiles < sms ? tiles : sms), kThreads, GemmLayout<false>::kSmem, (cudaStream_t)stream>>>(a);
-    e = cudaGetLastError();
-  }
+  if ((rc = pairs ? configure_smem<fp8_gemm_kernel<true>>(GemmLayout<true>::kSmem)
+                  : configure_smem<fp8_gemm_kernel<false>>(GemmLayout<false>::kSmem))) return rc;
+  const int most = pairs ? sms / 2 : sms, size = pairs ? 2 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(size * (tiles < most ? tiles : most)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = pairs ? GemmLayout<true>::kSmem : GemmLayout<false>::kSmem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = quantise ? 2 : 1;
+  cudaError_t e = pairs ? cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<true>, a) : cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<false>, a);
   if (e != cudaSuccess) return cuda_fail(e, "fp8_gemm_kernel launch");
   return XDIT_OK;
 }
