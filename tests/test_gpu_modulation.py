@@ -113,6 +113,29 @@ def test_every_combination(B, s, C, how, norm, post):
     _check(_rand((B, s, C), torch.bfloat16, 12), _rand((B, s, C), torch.bfloat16, 13), **o)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("C", [2, 130, 234, 235, 386, 387, 766, 769, 770, 1537, 2562, 10002])
+def test_widths_by_pairs_and_by_values(C, dtype):
+    """Widths that 16-byte words do not fit, at both ends of every way that they are split over threads."""
+    x, y = _rand((3, 7, C), dtype, 30, 2.0, 0.5), _rand((3, 7, C), dtype, 31)
+    for vec in {dtype, torch.float32}:
+        _check(x, y, **_options(3, 7, C, vec, "batch", "layer", "rms"))
+        _check(x, y, **_options(3, 7, C, vec, "token", "rms", None))
+
+
+@pytest.mark.parametrize("C", [234, 1152])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("which", ["x", "branch", "scale"])
+def test_one_operand_off_its_words(which, offset, C):
+    """One operand starts between words: all of them go by pairs, or by values where the start is odd."""
+    def at(shape, dtype, seed, off):
+        return _rand((*shape[:-1], shape[-1] + 8), dtype, seed)[..., off:off + shape[-1]]
+    x = at((2, 5, C), torch.bfloat16, 32, offset if which == "x" else 0)
+    y = at((2, 5, C), torch.bfloat16, 33, offset if which == "branch" else 0)
+    scale = at((2, 1, C), torch.float32, 34, offset if which == "scale" else 0)
+    _check(x, y, scale=scale, shift=_rand((2, 1, C), torch.float32, 35), norm="layer")
+
+
 @pytest.mark.parametrize("s", [1, 2, 149, 5000])
 def test_modulated_norm_alone(s):
     C = 1152

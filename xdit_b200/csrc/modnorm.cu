@@ -75,7 +75,7 @@ template <> struct Word<__half> {
   }
 };
 
-// The arithmetic runs on packed pairs (V = 8) or on single values (V = 1).
+// The arithmetic runs on packed pairs, or on single values (V = 1).
 template <int V> struct Lane { using E = uint64_t; static constexpr int N = V / 2; };
 template <> struct Lane<1> { using E = float; static constexpr int N = 1; };
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -112,7 +112,9 @@ __device__ __forceinline__ float total(uint64_t x) {
 }
 __device__ __forceinline__ float total(float x) { return x; }
 
-// V consecutive values as they lie in memory: V = 8 in 16-byte words, V = 1 alone.
+// V consecutive values as they lie in memory: V = 8 in 16-byte words, V = 2 in one access, V = 1 alone.
+template <int BYTES> struct Pair { using type = uint32_t; };
+template <> struct Pair<4> { using type = float2; };
 template <typename T, int V> struct Raw {
   static constexpr int kWords = V * sizeof(T) / 16;
   uint4 w[kWords];
@@ -150,6 +152,25 @@ template <typename T, int V> struct Raw {
       if constexpr (sizeof(T) == 4) { u[2 * i] = __float_as_uint(lo); u[2 * i + 1] = __float_as_uint(hi); }
       else u[i] = Word<T>::put(lo, hi);
     }
+  }
+};
+template <typename T> struct Raw<T, 2> {  // two values in one word (16 bits each) or two
+  using W = typename Pair<sizeof(T)>::type;
+  W w;
+  __device__ __forceinline__ void load_once(const T* p) { w = *reinterpret_cast<const W*>(p); }
+  __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const W*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
+  __device__ __forceinline__ void get(uint64_t (&x)[1]) const {
+    float lo, hi;
+    if constexpr (sizeof(T) == 4) { lo = w.x; hi = w.y; }
+    else Word<T>::get(w, lo, hi);
+    x[0] = pair(lo, hi);
+  }
+  __device__ __forceinline__ void put(const uint64_t (&x)[1]) {
+    float lo, hi;
+    split(x[0], lo, hi);
+    if constexpr (sizeof(T) == 4) w = make_float2(lo, hi);
+    else w = Word<T>::put(lo, hi);
   }
 };
 template <typename T> struct Raw<T, 1> {
@@ -462,7 +483,8 @@ cudaError_t launch(const NormArgs& a, int sms, cudaStream_t stream) {
 }
 
 // Threads and vectors per thread of a row: as few threads as hold it in five vectors each (one warp up to
-// 1280 values: no barrier between a row's loads and its stores).  Rows that 16-byte words do not fit go value by value.
+// 1280 values: no barrier between a row's loads and its stores).  Rows that 16-byte words do not fit go by pairs of values
+// or, of odd width, value by value (190,568 rows of 234: 471 us by values in CTAs of 128, 145 us by pairs in warps).
 template <typename T>
 cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
 #define XDIT_VPT5(V, TPR)                                       \
@@ -479,14 +501,27 @@ cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
     XDIT_VPT5(8, 512)
   }
 #undef XDIT_VPT5
-  if (a.nvec <= 512) return launch<T, 1, 128, 4>(a, sms, stream);
-  if (a.nvec <= 1280) return launch<T, 1, 128, 10>(a, sms, stream);
+  if (V == 2) {
+    if (a.nvec <= 64) return launch<T, 2, 32, 2>(a, sms, stream);
+    if (a.nvec <= 160) return launch<T, 2, 32, 5>(a, sms, stream);
+    if (a.nvec <= 384) return launch<T, 2, 32, 12>(a, sms, stream);
+    if (a.nvec <= 1280) return launch<T, 2, 128, 10>(a, sms, stream);
+    return launch<T, 2, 512, 16>(a, sms, stream);
+  }
+  if (a.nvec <= 128) return launch<T, 1, 32, 4>(a, sms, stream);
+  if (a.nvec <= 384) return launch<T, 1, 32, 12>(a, sms, stream);
+  if (a.nvec <= 768) return launch<T, 1, 32, 24>(a, sms, stream);
+  if (a.nvec <= 1536) return launch<T, 1, 128, 12>(a, sms, stream);
   if (a.nvec <= 4096) return launch<T, 1, 512, 8>(a, sms, stream);
   return launch<T, 1, 512, 32>(a, sms, stream);
 }
 
-bool aligned_rows(const void* p, int64_t sb, int64_t srow, int es, const xdit_norm_params& q) {
-  return ((uintptr_t)p & 15) == 0 && (q.B == 1 || (sb * es) % 16 == 0) && (q.s == 1 || (srow * es) % 16 == 0);
+// Low bits of all that a row's vectors start from, in elements of `es` bytes: 0 in the bits that all have clear.
+uint64_t low_bits(const void* p, int64_t sb, int64_t srow, int es, const xdit_norm_params& q) {
+  uint64_t low = (uint64_t)(uintptr_t)p;
+  if (q.B > 1) low |= (uint64_t)(sb * es);
+  if (q.s > 1) low |= (uint64_t)(srow * es);
+  return low;
 }
 
 }  // namespace
@@ -512,11 +547,17 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
   }
   NormArgs a;
   memset(&a, 0, sizeof(a));
-  bool wide = p.C % 8 == 0;
-  wide &= aligned_rows(p.residual, p.residual_stride_b, p.residual_stride_row, es, p);
-  if (p.branch) wide &= aligned_rows(p.branch, p.branch_stride_b, p.branch_stride_row, es, p);
-  if (p.out_residual) wide &= aligned_rows(p.out_residual, p.out_residual_stride_b, p.out_residual_stride_row, es, p);
-  if (p.out && !p.out_q) wide &= aligned_rows(p.out, p.out_stride_b, p.out_stride_row, es, p);
+  // V = 8 takes 16-byte words everywhere, V = 2 the size of two elements
+  uint64_t low = 0, low_pair = 0;
+  auto look = [&](const void* ptr, int64_t sb, int64_t srow, int size) {
+    const uint64_t l = low_bits(ptr, sb, srow, size, p);
+    low |= l;
+    low_pair |= l & (uint64_t)(2 * size - 1);
+  };
+  look(p.residual, p.residual_stride_b, p.residual_stride_row, es);
+  if (p.branch) look(p.branch, p.branch_stride_b, p.branch_stride_row, es);
+  if (p.out_residual) look(p.out_residual, p.out_residual_stride_b, p.out_residual_stride_row, es);
+  if (p.out && !p.out_q) look(p.out, p.out_stride_b, p.out_stride_row, es);
   const xdit_row_vec* in[7] = {&p.post_weight, &p.post_bias, &p.gate, &p.weight, &p.bias, &p.scale, &p.shift};
   RowVec* to[7] = {&a.post_weight, &a.post_bias, &a.gate, &a.weight, &a.bias, &a.scale, &a.shift};
   for (int i = 0; i < 7; ++i) {
@@ -529,8 +570,10 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
     to[i]->stride_b = in[i]->stride_b;
     to[i]->stride_row = in[i]->stride_row;
     to[i]->f32 = in[i]->dtype == XDIT_F32;
-    wide &= aligned_rows(in[i]->ptr, in[i]->stride_b, in[i]->stride_row, dtype_size(in[i]->dtype), p);
+    look(in[i]->ptr, in[i]->stride_b, in[i]->stride_row, dtype_size(in[i]->dtype));
   }
+  const bool wide = p.C % 8 == 0 && (low & 15) == 0;
+  const int V = wide ? 8 : p.C % 2 == 0 && low_pair == 0 ? 2 : 1;
   if (p.out_q && (!wide || p.C % 16 || ((uintptr_t)p.out_q & 15) || p.out_scale_ld < (int64_t)p.B * p.s)) {
     set_error("%s: e4m3 rows need C %% 16 == 0, 16-byte aligned rows and out_scale_ld of at least B*s", who);
     return XDIT_E_ALIGN;
@@ -544,12 +587,12 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
   a.out_z = p.out; a.z_sb = p.out_stride_b; a.z_srow = p.out_stride_row;
   a.out_q = (uint8_t*)p.out_q; a.out_scale = p.out_scale; a.scale_ld = p.out_scale_ld;
   a.rows = p.B * p.s; a.s = p.s; a.C = p.C;
-  a.nvec = wide ? p.C / 8 : p.C;
+  a.nvec = p.C / V;
   a.post = p.post_norm; a.norm = p.norm;
   a.residual_scale = p.residual_scale; a.eps = p.eps;
-  cudaError_t e = p.dtype == XDIT_BF16  ? dispatch<__nv_bfloat16>(a, wide ? 8 : 1, sms, stream)
-                  : p.dtype == XDIT_F16 ? dispatch<__half>(a, wide ? 8 : 1, sms, stream)
-                                        : dispatch<float>(a, wide ? 8 : 1, sms, stream);
+  cudaError_t e = p.dtype == XDIT_BF16  ? dispatch<__nv_bfloat16>(a, V, sms, stream)
+                  : p.dtype == XDIT_F16 ? dispatch<__half>(a, V, sms, stream)
+                                        : dispatch<float>(a, V, sms, stream);
   if (e != cudaSuccess) return cuda_fail(e, "gated_residual_norm_kernel launch");
   return XDIT_OK;
 }
