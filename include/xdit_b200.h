@@ -384,7 +384,7 @@ XDIT_API int xdit_rotary_tables(const struct xdit_rotary_positions* pos, float* 
  * With out_q the second result is written as e4m3 rows instead of `out`: [B*s, C] bytes and one scale
  * for each block of 128, out_scale[block * out_scale_ld + row]; needs C % 16 == 0 and 16-byte aligned rows.
  * Replaces: norm1/norm2 + modulation + gated residual around the attention and the MLP of the blocks that
- * transformer_wan.py:321-336 and transformer_flux.py:300-330 run. */
+ * the reference's model wrappers run. */
 #define XDIT_NORM_MAX_C 16384
 #define XDIT_FP8_BLOCK 128
 enum xdit_norm_kind { XDIT_NORM_NONE = 0, XDIT_NORM_LAYER = 1, XDIT_NORM_RMS = 2 };

@@ -8,6 +8,9 @@
 // HBM-bound: residual and branch are read once, h and z written once; the row stays in registers (fp32,
 // unrounded) between the sums and the writes.  LayerNorm takes the mean first and then the squares of the
 // centred values, both from registers, so a row with a large mean loses nothing to cancellation.
+// 75,600 rows of 5120 in bf16 (3.10 GB) take 554-575 us (5.4-5.6 TB/s, 0.82-0.86 of a copy), 9450 rows 77.7 us.  A row
+// takes registers, so an SM holds 16 warps, and the row that each has on its way is what hides the latency (without it
+// 760 us).  CTAs of 128 threads, four on an SM: three 633, five 616 (spills), six 731; three of 256 threads 600.
 #include <cstring>
 
 #include "fp8_quant.cuh"
@@ -373,7 +376,8 @@ gated_residual_norm_kernel(const __grid_constant__ NormArgs a) {
 }
 
 // Rows of a tensor to e4m3 with one scale for each block of 128: a CTA walks whole rows, 16 threads hold a block, and
-// four vectors of a thread are on their way at a time.
+// four vectors of a thread are on their way at a time (HBM-bound: 75,600 x 5120 bf16, 1.16 GB, 192 us or 6.05 TB/s; one
+// vector at a time 280 us).
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
 quantize_rows_kernel(const T* x, int64_t sb, int64_t srow, int s, int64_t rows, int K, uint8_t* q, float* scale,
@@ -419,7 +423,7 @@ quantize_rows_kernel(const T* x, int64_t sb, int64_t srow, int s, int64_t rows, 
 }
 
 // A weight [N, K] to e4m3 with one scale for each block of 128 x 128: one CTA per block, which a thread
-// crosses in pieces of 8 columns.
+// crosses in pieces of 8 columns (run once for a weight, so left simple).
 template <typename T>
 __global__ void __launch_bounds__(256)
 quantize_weight_kernel(const T* w, int64_t srow, int N, int K, uint8_t* q, float* scale) {
@@ -483,8 +487,10 @@ cudaError_t launch(const NormArgs& a, int sms, cudaStream_t stream) {
 }
 
 // Threads and vectors per thread of a row: as few threads as hold it in five vectors each (one warp up to
-// 1280 values: no barrier between a row's loads and its stores).  Rows that 16-byte words do not fit go by pairs of values
-// or, of odd width, value by value (190,568 rows of 234: 471 us by values in CTAs of 128, 145 us by pairs in warps).
+// 1280 values: no barrier between a row's loads and its stores).  Rows that 16-byte words do not fit go by pairs of
+// values or, of odd width, value by value (190,568 rows of 234: 471 us by values in CTAs of 128, 145 us by pairs in warps,
+// 202 us of 235 by values), in threads enough for few registers: 6000 rows of 6002 take 137 us by 7 pairs a thread, 211 us by
+// 16 with the last ones idle; 3063 of 1155 by values 15.6 us by 10 a thread and 17.9 by 12.
 template <typename T>
 cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
 #define XDIT_VPT5(V, TPR)                                       \
@@ -505,13 +511,16 @@ cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
     if (a.nvec <= 64) return launch<T, 2, 32, 2>(a, sms, stream);
     if (a.nvec <= 160) return launch<T, 2, 32, 5>(a, sms, stream);
     if (a.nvec <= 384) return launch<T, 2, 32, 12>(a, sms, stream);
+    if (a.nvec <= 640) return launch<T, 2, 128, 5>(a, sms, stream);
     if (a.nvec <= 1280) return launch<T, 2, 128, 10>(a, sms, stream);
+    if (a.nvec <= 3584) return launch<T, 2, 512, 7>(a, sms, stream);
     return launch<T, 2, 512, 16>(a, sms, stream);
   }
   if (a.nvec <= 128) return launch<T, 1, 32, 4>(a, sms, stream);
   if (a.nvec <= 384) return launch<T, 1, 32, 12>(a, sms, stream);
   if (a.nvec <= 768) return launch<T, 1, 32, 24>(a, sms, stream);
-  if (a.nvec <= 1536) return launch<T, 1, 128, 12>(a, sms, stream);
+  if (a.nvec <= 1280) return launch<T, 1, 128, 10>(a, sms, stream);
+  if (a.nvec <= 2560) return launch<T, 1, 512, 5>(a, sms, stream);
   if (a.nvec <= 4096) return launch<T, 1, 512, 8>(a, sms, stream);
   return launch<T, 1, 512, 32>(a, sms, stream);
 }

@@ -2,8 +2,8 @@
 sub-layer that just ended and the modulated norm of the one that follows.
 
 It stands for ``hidden = hidden + gate * attn_output; normed = norm(hidden) * (1 + scale) + shift`` in the blocks that
-the reference's wrappers run (``transformer_wan.py:321-336``, ``transformer_flux.py:300-330``), for blocks with a second
-norm behind the sub-layer, and for the modulated norm alone.  Forward only, like everything in this package.
+the reference's wrappers run, for blocks with a second norm behind the sub-layer, and for the modulated norm alone.
+Forward only, like everything in this package.
 """
 from __future__ import annotations
 
