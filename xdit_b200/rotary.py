@@ -67,7 +67,7 @@ class RotaryEmbedding:
         if self.pairing not in ("interleaved", "halves"):
             raise ValueError(f"pairing {self.pairing!r}: 'interleaved' or 'halves'")
         f = self.frequencies
-        freq, axis, pairs = _pairs(tuple(self.axes_dim), self.theta, self.ladder, f if f is None else tuple(f))
+        freq, axis, pairs = _pairs(tuple(self.axes_dim), self.theta, self.ladder, f if f is None else tuple(map(float, f)))
         return ops.rotary_positions(freq, axis, pairs, len(self.axes_dim), positions=self.positions, grid=self.grid,
                                     start=self.start, batch=batch, rows=rows)
 
