@@ -227,3 +227,80 @@ def test_linear_c_entry_refuses(lib):
     assert lib.xdit_quantize_rows(None, 0, 0, 0, 1, 1, 32, 16, 16, 1, None) == -1
     assert lib.xdit_quantize_weight(16, 32, 0, 0, 32, 16, 16, None) == -2
     assert lib.xdit_quantize_weight(16, 36, 0, 2, 32, 16, 16, None) == -3
+
+
+# ---- outputs that could not take the result, sizes that 32 bits would take for others --------------------------------
+def test_e4m3_outputs_are_looked_at():
+    x, w = _rows(), _weight()
+    good_q, good_s = ops.empty_fp8_rows(3, 48, "cpu")
+    bad = [(torch.zeros(3, 48, dtype=torch.uint8), good_s, TypeError), (good_q, None, TypeError), (good_q, good_s.half(), TypeError),
+           (good_q[:2], good_s, ValueError), (good_q, good_s[:2], ValueError), (good_q, torch.ones(3, 2), ValueError),
+           (torch.zeros(3, 64).to(E4)[:, :48], good_s, ValueError)]
+    for q, s, error in bad:
+        with pytest.raises(error):
+            ops.fp8_linear(x.data, x.scale, w.data, w.scale, out_q=q, out_scale=s)
+        with pytest.raises(error):
+            ops.gated_residual_norm(torch.zeros(1, 3, 48), None, out_q=q, out_scale=s, norm="rms")
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.fp8_linear(x.data, x.scale, w.data, w.scale, out_q=good_q, out_scale=good_s)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Each of these would be a call of five rows if its size were cut to 32 bits."""
+    many = 2 ** 32 + 5
+    row = torch.zeros(16)
+    q = row.expand(1, 1, many, 16)
+    e = RotaryEmbedding((8, 8), grid=(1, 5))
+    with pytest.raises(ValueError, match="above"):
+        ops.rotary_axes(q, None, e._params(1, many), False, q, None)
+    with pytest.raises(ValueError, match="above"):
+        ops.rotary_axes(q.transpose(1, 2), None, e._params(1, 1), False, q.transpose(1, 2), None)
+    with pytest.raises(ValueError, match="above"):
+        ops.rotary_tables(e._params(1, many), many, 16, "cuda")
+    for x in (row.expand(1, many, 16), row.expand(2 ** 16, 2 ** 16 + 1, 16)):
+        with pytest.raises(ValueError, match="above"):
+            ops.gated_residual_norm(x, None, out=x, norm="rms")
+        with pytest.raises(ValueError, match="above"):
+            ops.fp8_linear(x, None, _weight(K=16).data, _weight(K=16).scale, out=row.expand(x.shape[0] * x.shape[1], 16))
+    with pytest.raises(ValueError, match="above"):
+        ops.quantize_rows(row.expand(1, many, 16))
+    with pytest.raises(ValueError, match="above"):
+        ops.quantize_weight(row.expand(many, 16))
+
+
+def test_c_entries_refuse_outputs_in_one_place_and_pointers_between_elements(lib):
+    f, a = (ctypes.c_double * 8)(), (ctypes.c_uint8 * 8)()
+    pair = ctypes.c_int64 * 2
+
+    def rotary(**kw):
+        p = _capi.RotaryParams(dtype=0, B=1, H=2, Hk=0, s=4, D=16, q=16, out_q=16, stride_h=pair(64, 64), stride_row=pair(16, 16),
+                               out_stride_h=pair(64, 64), out_stride_row=pair(16, 16),
+                               pos=_capi.RotaryPositions(kind=0, axes=1, pairs=8, frequencies=f, axis=a))
+        p.pos.grid[0] = 4
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return lib.xdit_rotary_axes(ctypes.byref(p), None)
+
+    assert rotary(out_stride_h=pair(0, 0)) == -2 and rotary(out_stride_row=pair(0, 0)) == -2 and rotary(B=2) == -2
+    assert rotary(Hk=2, k=32, out_k=16) == -2 and rotary(Hk=2, k=32, out_k=48, out_stride_row=pair(16, 0)) == -2
+    assert rotary(out_q=17) == -3
+
+    def norm(**kw):
+        p = _capi.NormParams(dtype=0, B=1, s=2, C=32, norm=1, residual=16, out=16, residual_stride_row=32, out_stride_row=32)
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return lib.xdit_gated_residual_norm(ctypes.byref(p), None)
+
+    both = dict(branch=16, branch_stride_row=32, out_residual=64, out_residual_stride_row=32)
+    assert norm(out_stride_row=0) == -2 and norm(B=2) == -2 and norm(**{**both, "out_residual_stride_row": 0}) == -2
+    assert norm(**{**both, "out_residual": 16}) == -2
+    assert norm(residual=17) == -3 and norm(out=17) == -3 and norm(scale=_capi.RowVec(ptr=18, dtype=2)) == -3
+
+    def linear(**kw):
+        p = _capi.Fp8LinearParams(M=2, N=16, K=128, x=16, w=16, x_stride_row=128, w_stride_row=128, x_scale=16, w_scale=16,
+                                  out=16, out_stride_row=16)
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return lib.xdit_fp8_linear(ctypes.byref(p), None)
+
+    assert linear(x_scale=18) == -3 and linear(w_scale=17) == -3 and linear(bias=17, bias_dtype=0) == -3

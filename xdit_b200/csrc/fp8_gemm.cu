@@ -932,6 +932,11 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
     set_error("%s: rows of x, w and out_q must start on 16-byte boundaries, out_scale_ld be at least M", who);
     return XDIT_E_ALIGN;
   }
+  if ((((uintptr_t)p->x_scale | (uintptr_t)p->w_scale | (uintptr_t)p->out_scale) & 3) ||
+      (p->bias && ((uintptr_t)p->bias & (dtype_size(p->bias_dtype) - 1)))) {
+    set_error("%s: scales or bias are not aligned to their elements", who);
+    return XDIT_E_ALIGN;
+  }
   if (p->raw && (p->x_scale_stride_row != 1 || p->x_stride_row != p->K || p->raw_s < 0 || (p->raw_s && p->M % p->raw_s))) {
     set_error("%s: x is quantised into contiguous rows with scales stored block by block; raw_s=%d of M=%d", who, p->raw_s, p->M);
     return XDIT_E_SHAPE;

@@ -558,10 +558,12 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
   memset(&a, 0, sizeof(a));
   // V = 8 takes 16-byte words everywhere, V = 2 the size of two elements
   uint64_t low = 0, low_pair = 0;
+  bool off = false;  // a pointer between elements
   auto look = [&](const void* ptr, int64_t sb, int64_t srow, int size) {
     const uint64_t l = low_bits(ptr, sb, srow, size, p);
     low |= l;
     low_pair |= l & (uint64_t)(2 * size - 1);
+    off |= ((uintptr_t)ptr & (size - 1)) != 0;
   };
   look(p.residual, p.residual_stride_b, p.residual_stride_row, es);
   if (p.branch) look(p.branch, p.branch_stride_b, p.branch_stride_row, es);
@@ -580,6 +582,13 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
     to[i]->stride_row = in[i]->stride_row;
     to[i]->f32 = in[i]->dtype == XDIT_F32;
     look(in[i]->ptr, in[i]->stride_b, in[i]->stride_row, dtype_size(in[i]->dtype));
+  }
+  if (off) { set_error("%s: a pointer is not aligned to its elements", who); return XDIT_E_ALIGN; }
+  const bool h_one = p.out_residual && ((p.B > 1 && !p.out_residual_stride_b) || (p.s > 1 && !p.out_residual_stride_row));
+  const bool z_one = p.out && !p.out_q && ((p.B > 1 && !p.out_stride_b) || (p.s > 1 && !p.out_stride_row));
+  if (h_one || z_one || (p.norm != XDIT_NORM_NONE && p.out && p.out == p.out_residual)) {
+    set_error("%s: an output holds several rows in one place, or both outputs are one", who);
+    return XDIT_E_SHAPE;
   }
   const bool wide = p.C % 8 == 0 && (low & 15) == 0;
   const int V = wide ? 8 : p.C % 2 == 0 && low_pair == 0 ? 2 : 1;

@@ -300,8 +300,6 @@ int launch_rotary(const xdit_rotary_params& p, cudaStream_t stream) {
   }
   if (p.B == 0 || p.s == 0) return XDIT_OK;
   if (!p.q || !p.out_q || (p.Hk && (!p.k || !p.out_k))) { set_error("xdit_rotary_axes: NULL q, k or output"); return XDIT_E_NULL; }
-  int sms = 0;
-  if ((rc = check_device(&sms))) return rc;
   const int halves = p.halves != 0;
   a.src[0] = (const char*)p.q; a.src[1] = (const char*)p.k;
   a.dst[0] = (char*)p.out_q; a.dst[1] = (char*)p.out_k;
@@ -317,7 +315,15 @@ int launch_rotary(const xdit_rotary_params& p, cudaStream_t stream) {
     if (a.heads[t] > 1) low |= (uint64_t)(a.ss_h[t] | a.ds_h[t]) * es;
     if (p.s > 1) low |= (uint64_t)(a.ss_row[t] | a.ds_row[t]) * es;
   }
+  for (int t = 0; t < (p.Hk ? 2 : 1); ++t)
+    if ((p.B > 1 && !a.ds_b[t]) || (a.heads[t] > 1 && !a.ds_h[t]) || (p.s > 1 && !a.ds_row[t])) {
+      set_error("xdit_rotary_axes: an output holds several tokens or heads in one place");
+      return XDIT_E_SHAPE;
+    }
+  if (p.Hk && p.out_q == p.out_k) { set_error("xdit_rotary_axes: q and k have one output"); return XDIT_E_SHAPE; }
   if (low % es) { set_error("xdit_rotary_axes: a pointer is not aligned to its elements"); return XDIT_E_ALIGN; }
+  int sms = 0;
+  if ((rc = check_device(&sms))) return rc;
   int V = 16 / es;
   const int whole = halves ? a.rot / 2 : a.rot;
   while (V > 1 && ((low % (V * es)) || whole % V || (p.D - a.rot) % V)) V /= 2;

@@ -607,6 +607,24 @@ def _launch(fn, t: torch.Tensor, where: str, *args) -> None:
         _capi.check(rc, where)
 
 
+_MOST = 0x7fffffff
+
+
+def _counted(*sizes: int) -> None:
+    """The C entries count samples, rows, heads and values in 32 bits; a size that they would take for another is refused."""
+    if max(sizes) > _MOST:
+        raise ValueError(f"a size above {_MOST} in {sizes}")
+
+
+def _e4m3_out(q: torch.Tensor, scale: Optional[torch.Tensor], rows: int, K: int) -> None:
+    """``q`` and ``scale`` can take ``rows`` e4m3 rows of ``K`` values and their scales."""
+    kb = -(-K // _capi.XDIT_FP8_BLOCK)
+    if scale is None or q.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
+        raise TypeError("e4m3 rows go to a float8_e4m3fn tensor and their scales to an fp32 one")
+    if q.shape != (rows, K) or not q.is_contiguous() or scale.shape != (rows, kb):
+        raise ValueError(f"e4m3 rows {tuple(q.shape)} with scales {tuple(scale.shape)} for a result of {(rows, K)}")
+
+
 def _rows_contiguous(t: torch.Tensor, name: str) -> None:
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         raise ValueError(f"the last axis of {name} must be contiguous")
@@ -656,6 +674,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.Rot
         raise ValueError("q, k and their outputs must agree in B, s and D")
     if 2 * positions.pairs > D:
         raise ValueError(f"{2 * positions.pairs} elements to rotate in a head of {D}")
+    _counted(B, H, s, D, 0 if k is None else k.shape[1])
     qb, qh, qs, q1 = q.stride()
     ob, oh, os_, o1 = out_q.stride()
     kb = kh = ks = pb = ph = ps = Hk = 0
@@ -678,6 +697,7 @@ def rotary_tables(positions: _capi.RotaryPositions, s: int, D: int, device) -> t
     """``(cos, sin)``, fp32 ``[s, D]``, of the interleaved pairs at ``positions``: the tables that
     :func:`qk_norm_rope_pack` takes (``xdit_rotary_tables``)."""
     global launch_count
+    _counted(s)
     device = torch.device(device)
     if device.type != "cuda":
         raise RuntimeError(f"xdit_b200 kernels run on CUDA devices only (sm_100a), not on {device}. There is no CPU fallback.")
@@ -749,6 +769,9 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], 
     x = residual
     dtype = _dtype(x)
     B, s, Cn = x.shape
+    _counted(B * s, Cn)
+    if out_q is not None:
+        _e4m3_out(out_q, out_scale, B * s, Cn)
     r, y = _rows(x, x, "residual"), _rows(branch, x, "branch")
     oh, oz = _rows(out_residual, x, "out_residual"), _rows(out, x, "out")
     rows = (_row_vec(post_weight, x, "post_weight", True), _row_vec(post_bias, x, "post_bias", True),
@@ -786,6 +809,7 @@ def quantize_rows(x: torch.Tensor) -> tuple:
     B, s, K = x.shape
     if K % 16 or K == 0:
         raise ValueError(f"rows of {K} values: a multiple of 16 is needed")
+    _counted(B, s, K)
     dt = _dtype(x)
     _rows_contiguous(x, "x")
     _check_tensors(x)
@@ -802,6 +826,7 @@ def quantize_weight(w: torch.Tensor) -> tuple:
     global launch_count
     if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 16 or w.shape[1] % 16:
         raise ValueError(f"a weight [N, K] with K a multiple of 16 is needed, got {tuple(w.shape)}")
+    _counted(*w.shape)
     dt = _dtype(w)
     _rows_contiguous(w, "w")
     _check_tensors(w)
@@ -839,6 +864,7 @@ def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor
     M = x.shape[0] if given else x.shape[0] * x.shape[1]
     if K % 16 or K == 0 or N == 0:
         raise ValueError(f"K = {K}: a multiple of 16 is needed (and N = {N} rows of the weight)")
+    _counted(M, N, K)
     kb, nb = (K + 127) // 128, (N + 127) // 128
     if w_scale.shape != (nb, kb) or (given and x_scale.shape != (M, kb)):
         raise ValueError(f"scales of other shapes than {(M, kb)} and {(nb, kb)} for rows {tuple(x.shape)} and a weight {tuple(w.shape)}")
@@ -863,6 +889,7 @@ def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor
     else:
         if N % 16:
             raise ValueError(f"e4m3 rows of {N} values: a multiple of 16 is needed")
+        _e4m3_out(out_q, out_scale, M, N)
         o = (None, 0, out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale))
     b = (bias.data_ptr(), _dtype(bias)) if bias is not None else (None, 0)
     raw = (0, 0, None, 0, 0)
