@@ -136,6 +136,17 @@ def test_one_operand_off_its_words(which, offset, C):
     _check(x, y, scale=scale, shift=_rand((2, 1, C), torch.float32, 35), norm="layer")
 
 
+@pytest.mark.parametrize("C", [64, 1152, 5120])
+@pytest.mark.parametrize("offset", [0, 4, 8, 12])
+def test_modulation_in_fp32_at_16_and_32_byte_boundaries(offset, C):
+    """Rows of modulation that start on 16-byte words, and those on 32-byte ones, for all, for samples and for tokens."""
+    x, y = _rand((2, 7, C), torch.bfloat16, 36), _rand((2, 7, C), torch.bfloat16, 37)
+    for shape, step in (((C,), 0), ((2, 1, C), 4), ((2, 7, C), 8)):
+        def at(seed):
+            return _rand((*shape[:-1], C + 16 + step), torch.float32, seed)[..., offset:offset + C]
+        _check(x, y, gate=at(38), scale=at(39), shift=at(40), post_norm="rms", post_weight=_rand((C,), torch.float32, 41), norm="layer")
+
+
 @pytest.mark.parametrize("s", [1, 2, 149, 5000])
 def test_modulated_norm_alone(s):
     C = 1152

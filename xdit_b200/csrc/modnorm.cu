@@ -8,9 +8,11 @@
 // HBM-bound: residual and branch are read once, h and z written once; the row stays in registers (fp32,
 // unrounded) between the sums and the writes.  LayerNorm takes the mean first and then the squares of the
 // centred values, both from registers, so a row with a large mean loses nothing to cancellation.
-// 75,600 rows of 5120 in bf16 (3.10 GB) take 554-575 us (5.4-5.6 TB/s, 0.82-0.86 of a copy), 9450 rows 77.7 us.  A row
-// takes registers, so an SM holds 16 warps, and the row that each has on its way is what hides the latency (without it
-// 760 us).  CTAs of 128 threads, four on an SM: three 633, five 616 (spills), six 731; three of 256 threads 600.
+// 75,600 rows of 5120 in bf16 with modulation in fp32 (3.10 GB) take 500 us (6.2 TB/s, 0.94 of a copy).  A row takes
+// registers, so an SM holds 16 warps, and the row that each has on its way is what hides the latency (without it
+// 760 us).  CTAs of 128 threads, four on an SM: three 633, five 616 (spills), six 731; three of 256 threads 600.  The
+// modulation's 60 KB a row come from L1, more bytes than the row's own 40 KB: 551 us while they came 16 bytes a load,
+// 610-637 with the row ahead in shared memory (five or six CTAs on an SM), which takes L1's room.
 #include <cstring>
 
 #include "fp8_quant.cuh"
@@ -23,7 +25,7 @@ constexpr int kQuantThreads = 160;
 struct RowVec {  // a row of C values: the same for all, or with a stride for samples or tokens
   const void* ptr;
   int64_t stride_b, stride_row;
-  int32_t f32;
+  int32_t f32;  // 0: in the tensors' dtype, 1: fp32, 2: fp32 and every vector on a 32-byte boundary
 };
 
 struct NormArgs {
@@ -132,6 +134,14 @@ template <typename T, int V> struct Raw {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   }
+  // 32 bytes of a modulation row from a 32-byte boundary, in one load (two loads of 16 bytes lie 32 apart from thread to
+  // thread and pass L1 at half the rate)
+  __device__ __forceinline__ void load_wide(const T* p) {
+    static_assert(kWords == 2);
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y), "=r"(w[1].z), "=r"(w[1].w)
+        : "l"(p));
+  }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) *(reinterpret_cast<uint4*>(p) + i) = w[i];
@@ -187,14 +197,15 @@ template <typename T> struct Raw<T, 1> {
 
 enum { kAdd, kMul, kScale };
 // x (op) the modulation row `v`, which starts at element `at` for this thread: x + v, x v, x (1 + v).
-template <int OP, typename R, int V, int TPR, int VPT, typename E>
+template <int OP, typename R, bool WIDE, int V, int TPR, int VPT, typename E>
 __device__ __forceinline__ void apply_as(const void* ptr, int64_t at, int t, int nvec, E (&x)[VPT][Lane<V>::N]) {
   const R* p = reinterpret_cast<const R*>(ptr) + at;
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     if (t + TPR * k >= nvec) continue;
     Raw<R, V> raw;
-    raw.load(p + TPR * k * V);
+    if constexpr (WIDE) raw.load_wide(p + TPR * k * V);
+    else raw.load(p + TPR * k * V);
     E v[Lane<V>::N];
     raw.get(v);
 #pragma unroll
@@ -206,8 +217,13 @@ template <int OP, typename T, int V, int TPR, int VPT, typename E>
 __device__ __forceinline__ void apply(const RowVec& v, int b, int row, int t, int nvec, E (&x)[VPT][Lane<V>::N]) {
   if (!v.ptr) return;
   const int64_t at = b * v.stride_b + row * v.stride_row + t * V;
-  if (v.f32) apply_as<OP, float, V, TPR, VPT>(v.ptr, at, t, nvec, x);
-  else apply_as<OP, T, V, TPR, VPT>(v.ptr, at, t, nvec, x);
+  if (v.f32 == 2) {
+    if constexpr (V == 8) apply_as<OP, float, true, V, TPR, VPT>(v.ptr, at, t, nvec, x);
+  } else if (v.f32) {
+    apply_as<OP, float, false, V, TPR, VPT>(v.ptr, at, t, nvec, x);
+  } else {
+    apply_as<OP, T, false, V, TPR, VPT>(v.ptr, at, t, nvec, x);
+  }
 }
 
 // Sum over the TPR threads of a row.  The shared buffer alternates, so one barrier per sum is enough: a
@@ -580,7 +596,8 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
     to[i]->ptr = in[i]->ptr;
     to[i]->stride_b = in[i]->stride_b;
     to[i]->stride_row = in[i]->stride_row;
-    to[i]->f32 = in[i]->dtype == XDIT_F32;
+    const bool apart = (low_bits(in[i]->ptr, in[i]->stride_b, in[i]->stride_row, 4, p) & 31) != 0;
+    to[i]->f32 = in[i]->dtype != XDIT_F32 ? 0 : apart ? 1 : 2;
     look(in[i]->ptr, in[i]->stride_b, in[i]->stride_row, dtype_size(in[i]->dtype));
   }
   if (off) { set_error("%s: a pointer is not aligned to its elements", who); return XDIT_E_ALIGN; }
@@ -591,6 +608,8 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
     return XDIT_E_SHAPE;
   }
   const bool wide = p.C % 8 == 0 && (low & 15) == 0;
+  if (!wide)
+    for (RowVec* v : to) v->f32 = v->f32 != 0;  // 32 bytes are the width of V = 8
   const int V = wide ? 8 : p.C % 2 == 0 && low_pair == 0 ? 2 : 1;
   if (p.out_q && (!wide || p.C % 16 || ((uintptr_t)p.out_q & 15) || p.out_scale_ld < (int64_t)p.B * p.s)) {
     set_error("%s: e4m3 rows need C %% 16 == 0, 16-byte aligned rows and out_scale_ld of at least B*s", who);
