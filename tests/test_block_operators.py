@@ -304,3 +304,19 @@ def test_c_entries_refuse_outputs_in_one_place_and_pointers_between_elements(lib
         return lib.xdit_fp8_linear(ctypes.byref(p), None)
 
     assert linear(x_scale=18) == -3 and linear(w_scale=17) == -3 and linear(bias=17, bias_dtype=0) == -3
+
+
+def test_packed_parameters_are_the_structures_bytes():
+    f, a = (ctypes.c_double * 8)(), (ctypes.c_uint8 * 8)()
+    pos = _capi.RotaryPositions(2, 3, 8, f, a, 123456, 7, 8, 9, (5, 6, 7, 8), 11)
+    pair = ctypes.c_int64 * 2
+    want = _capi.RotaryParams(2, 3, 4, 5, 6, 7, True, pos, 2 ** 63 + 1, 12, 13, 0, *(pair(i, -i) for i in range(6)))
+    got = _capi.pack_rotary(2, 3, 4, 5, 6, 7, True, bytes(pos), 2 ** 63 + 1, 12, 13, 0, *(j for i in range(6) for j in (i, -i)))
+    assert got == bytes(want)
+    rows = [(1000 + i, i, 2 * i, i % 3) for i in range(7)]
+    head = (1, 2, 3, 4, 2, 1, 0.75, 1e-6, *range(20, 35))
+    assert _capi.pack_norm(*head, *(v for r in rows for v in r)) == bytes(_capi.NormParams(*head, *rows))
+    n = len(_capi.Fp8LinearParams._fields_)
+    assert _capi.pack_fp8_linear(*range(n)) == bytes(_capi.Fp8LinearParams(*range(n)))
+    with pytest.raises(Exception):
+        _capi.pack_fp8_linear(2 ** 32 + 5, *range(1, n))

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 # XDIT_B200_LIB selects another build of the same library (same ABI), e.g. one compiled with other options
@@ -189,6 +190,38 @@ class Fp8LinearParams(C.Structure):
     ]
 
 
+_CODES = {C.c_int32: "i", C.c_uint32: "I", C.c_int64: "q", C.c_float: "f", C.c_void_p: "Q"}
+
+
+def _format(struct_type, whole=()) -> str:
+    out, at = [], 0
+    for name, kind in struct_type._fields_:
+        field = getattr(struct_type, name)
+        out.append("x" * (field.offset - at))
+        at = field.offset + field.size
+        if kind in whole:
+            out.append(f"{field.size}s")
+        elif issubclass(kind, C.Structure):
+            out.append(_format(kind, whole))
+        elif issubclass(kind, C.Array):
+            out.append(_CODES[kind._type_] * kind._length_)
+        else:
+            out.append(_CODES[kind])
+    return "".join(out) + "x" * (C.sizeof(struct_type) - at)
+
+
+def packer(struct_type, *whole) -> struct.Struct:
+    """Packs the fields of ``struct_type``, in order, with nested structures and arrays taken apart (those of the types
+    ``whole`` as bytes) and 0 for NULL, into the bytes that its entry point reads.  For the calls of a few microseconds: a
+    ctypes structure of thirty fields takes 5 us to fill, these bytes less than one, and a number that its field cannot
+    hold raises."""
+    return struct.Struct("=" + _format(struct_type, whole))
+
+
+pack_rotary = packer(RotaryParams, RotaryPositions).pack
+pack_norm = packer(NormParams).pack
+pack_fp8_linear = packer(Fp8LinearParams).pack
+
 _lib = None
 
 
@@ -261,12 +294,12 @@ def load() -> C.CDLL:
     lib.xdit_merge_out_lse.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
     lib.xdit_merge_out_lse.restype = C.c_int
-    lib.xdit_rotary_axes.argtypes = [C.POINTER(RotaryParams), C.c_void_p]
+    lib.xdit_rotary_axes.argtypes = [C.c_void_p, C.c_void_p]  # the structure, or its bytes
     lib.xdit_rotary_axes.restype = C.c_int
     lib.xdit_rotary_tables.argtypes = [C.POINTER(RotaryPositions), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                        C.c_void_p]
     lib.xdit_rotary_tables.restype = C.c_int
-    lib.xdit_gated_residual_norm.argtypes = [C.POINTER(NormParams), C.c_void_p]
+    lib.xdit_gated_residual_norm.argtypes = [C.c_void_p, C.c_void_p]
     lib.xdit_gated_residual_norm.restype = C.c_int
     lib.xdit_quantize_rows.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
@@ -274,7 +307,7 @@ def load() -> C.CDLL:
     lib.xdit_quantize_weight.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                          C.c_void_p, C.c_void_p]
     lib.xdit_quantize_weight.restype = C.c_int
-    lib.xdit_fp8_linear.argtypes = [C.POINTER(Fp8LinearParams), C.c_void_p]
+    lib.xdit_fp8_linear.argtypes = [C.c_void_p, C.c_void_p]
     lib.xdit_fp8_linear.restype = C.c_int
     _lib = lib
     return lib

@@ -189,11 +189,12 @@ def _launch_attn(fn, p, q, where):
     """Call an attention entry point; a timeout reported by an earlier launch surfaces here, and the
     status words are cleared so that the caller may retry."""
     device = q.get_device()
+    p = p if isinstance(p, bytes) else C.byref(p)
     if device == torch._C._cuda_getDevice():
-        rc = fn(C.byref(p), torch._C._cuda_getCurrentRawStream(device))
+        rc = fn(p, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(C.byref(p), torch._C._cuda_getCurrentRawStream(device))
+            rc = fn(p, torch._C._cuda_getCurrentRawStream(device))
     if rc == -6:  # XDIT_E_KERNEL_TIMEOUT
         msg = _capi.load().xdit_last_error_string()
         torch.cuda.synchronize(q.device)
@@ -657,7 +658,6 @@ def rotary_positions(frequencies, axis, pairs: int, axes: int, *, positions: Opt
                                  stride[0] if each and shape[0] > 1 else 0, stride[-2], stride[-1])
 
 
-_PAIR = C.c_int64 * 2
 _GRID = C.c_int64 * _capi.XDIT_ROTARY_MAX_AXES
 
 
@@ -677,8 +677,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.Rot
     _counted(B, H, s, D, 0 if k is None else k.shape[1])
     qb, qh, qs, q1 = q.stride()
     ob, oh, os_, o1 = out_q.stride()
-    kb = kh = ks = pb = ph = ps = Hk = 0
-    k_ptr = out_k_ptr = None
+    kb = kh = ks = pb = ph = ps = Hk = k_ptr = out_k_ptr = 0
     k1 = p1 = 1
     if k is not None:
         Hk, k_ptr, out_k_ptr = k.shape[1], k.data_ptr(), out_k.data_ptr()
@@ -687,9 +686,9 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: _capi.Rot
     if D != 1 and (q1 != 1 or o1 != 1 or k1 != 1 or p1 != 1):
         raise ValueError("the last axis of q, k and their outputs must be contiguous")
     _check_tensors(q, k, out_q, out_k)
-    p = _capi.RotaryParams(dtype, B, H, Hk, s, D, halves, positions, q.data_ptr(), k_ptr, out_q.data_ptr(), out_k_ptr,
-                           _PAIR(qb, kb), _PAIR(qh, kh), _PAIR(qs, ks), _PAIR(ob, pb), _PAIR(oh, ph), _PAIR(os_, ps))
-    _launch(_capi.load().xdit_rotary_axes, q, "xdit_rotary_axes", C.byref(p))
+    p = _capi.pack_rotary(dtype, B, H, Hk, s, D, halves, bytes(positions), q.data_ptr(), k_ptr, out_q.data_ptr(), out_k_ptr,
+                          qb, kb, qh, kh, qs, ks, ob, pb, oh, ph, os_, ps)
+    _launch(_capi.load().xdit_rotary_axes, q, "xdit_rotary_axes", p)
     launch_count += 1
 
 
@@ -731,14 +730,14 @@ def _row_vec(t: Optional[torch.Tensor], x: torch.Tensor, name: str, shared: bool
     return t.data_ptr(), sb, srow, _DTYPES[dtype]
 
 
-_NO_ROW = (None, 0, 0, 0)
+_NO_ROW = (0, 0, 0, 0)
 
 
 def _rows(t: Optional[torch.Tensor], x: torch.Tensor, name: str) -> tuple:
     """``(address, batch stride, row stride)`` of a tensor shaped like ``x`` [B, s, C]."""
     if t is None:
-        return None, 0, 0
-    if t.shape != x.shape:
+        return 0, 0, 0
+    if t is not x and t.shape != x.shape:
         raise ValueError(f"{name} {tuple(t.shape)} beside a residual {tuple(x.shape)}")
     if t.dtype is not x.dtype:
         raise TypeError(f"{name} must have the residual's dtype")
@@ -774,14 +773,14 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], 
         _e4m3_out(out_q, out_scale, B * s, Cn)
     r, y = _rows(x, x, "residual"), _rows(branch, x, "branch")
     oh, oz = _rows(out_residual, x, "out_residual"), _rows(out, x, "out")
-    rows = (_row_vec(post_weight, x, "post_weight", True), _row_vec(post_bias, x, "post_bias", True),
-            _row_vec(gate, x, "gate"), _row_vec(weight, x, "weight", True), _row_vec(bias, x, "bias", True),
-            _row_vec(scale, x, "scale"), _row_vec(shift, x, "shift"))
+    rows = (*_row_vec(post_weight, x, "post_weight", True), *_row_vec(post_bias, x, "post_bias", True),
+            *_row_vec(gate, x, "gate"), *_row_vec(weight, x, "weight", True), *_row_vec(bias, x, "bias", True),
+            *_row_vec(scale, x, "scale"), *_row_vec(shift, x, "shift"))
     _check_tensors(x, branch, out_residual, out, out_q, out_scale, gate, post_weight, post_bias, weight, bias, scale, shift)
-    q = (out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)) if out_q is not None else (None, None, 0)
-    p = _capi.NormParams(dtype, B, s, Cn, _NORMS[post_norm], _NORMS[norm], residual_scale, eps, r[0], y[0], r[1], r[2],
-                         y[1], y[2], oh[0], oz[0], oh[1], oh[2], oz[1], oz[2], *q, *rows)
-    _launch(_capi.load().xdit_gated_residual_norm, x, "xdit_gated_residual_norm", C.byref(p))
+    q = (out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale)) if out_q is not None else (0, 0, 0)
+    p = _capi.pack_norm(dtype, B, s, Cn, _NORMS[post_norm], _NORMS[norm], residual_scale, eps, r[0], y[0], r[1], r[2],
+                        y[1], y[2], oh[0], oz[0], oh[1], oh[2], oz[1], oz[2], *q, *rows)
+    _launch(_capi.load().xdit_gated_residual_norm, x, "xdit_gated_residual_norm", p)
     launch_count += 1
 
 
@@ -878,21 +877,20 @@ def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor
     xs = x.stride()
     if (ws1 != 1 or xs[-1] != 1) and K != 1:
         raise ValueError("the last axis of x and w must be contiguous")
-    o = (None, 0, None, None, 0)
     out_dtype = 0
     if out is not None:
         if out.shape != (M, N):
             raise ValueError(f"out {tuple(out.shape)} for a result of {(M, N)}")
         _rows_contiguous(out, "out")
         out_dtype = _dtype(out)
-        o = (out.data_ptr(), out.stride(0), None, None, 0)
+        o = (out.data_ptr(), out.stride(0), 0, 0, 0)
     else:
         if N % 16:
             raise ValueError(f"e4m3 rows of {N} values: a multiple of 16 is needed")
         _e4m3_out(out_q, out_scale, M, N)
-        o = (None, 0, out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale))
-    b = (bias.data_ptr(), _dtype(bias)) if bias is not None else (None, 0)
-    raw = (0, 0, None, 0, 0)
+        o = (0, 0, out_q.data_ptr(), out_scale.data_ptr(), _scale_ld(out_scale))
+    b = (bias.data_ptr(), _dtype(bias)) if bias is not None else (0, 0)
+    raw = (0, 0, 0, 0, 0)
     if not given:
         raw = (_dtype(x), x.shape[1], x.data_ptr(), xs[0], xs[1])
     _check_tensors(x, x_scale, w, w_scale, bias, out, out_q, out_scale)
@@ -903,7 +901,7 @@ def fp8_linear(x: torch.Tensor, x_scale: Optional[torch.Tensor], w: torch.Tensor
         scale_row, scale_block = 1, M
     address = rows.data_ptr()
     st = _status(x.device)
-    p = _capi.Fp8LinearParams(M, N, K, _ACTIVATIONS[activation], out_dtype, b[1], address, w.data_ptr(), xs[0] if given else K,
+    p = _capi.pack_fp8_linear(M, N, K, _ACTIVATIONS[activation], out_dtype, b[1], address, w.data_ptr(), xs[0] if given else K,
                               ws0, scales.data_ptr() if given else address + (M * K + 15) // 16 * 16, w_scale.data_ptr(),
                               scale_row, scale_block, *w_scale.stride(), b[0], *o, st.dev.data_ptr(), st.host.data_ptr(),
                               _wait_limit_ns, *raw, _selftest_stall)
