@@ -86,6 +86,26 @@ def test_model_sizes(M, N, K):
     _check(_rows(M, K, 7, columns=True), _weight(N, K, 8), torch.randn(N, device="cuda", generator=_gen(9)))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(65, 352, 6528), (129, 1000, 2064), (273, 352, 6528), (509, 130, 4096), (1000, 16, 2048)])
+def test_few_tiles_of_a_long_inner_axis(M, N, K, dtype):
+    """More rows than one tile of the kernel for few rows, the inner axis shared by a cluster: the last tile is a part."""
+    x, w = _rows(M, K, 50, columns=True), _weight(N, K, 51)
+    _check(x, w, torch.randn(N, device="cuda", generator=_gen(52)), "gelu_tanh" if M % 2 else None, dtype)
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 4608, 1040), (16, 2304, 2064), (64, 9216, 1024), (3, 1536, 4096), (2, 20000, 528)])
+def test_every_way_that_few_rows_are_split(M, N, K):
+    _check(_rows(M, K, 53, columns=True), _weight(N, K, 54), torch.randn(N, device="cuda", generator=_gen(55)))
+    if N % 16 == 0:
+        x, w = _rows(M, K, 53), _weight(N, K, 54)
+        r = fp8_linear(x, w, quantize_out=True)
+        want, tol = _want(x, w, None, None)
+        s = r.scale.double().repeat_interleave(128, 1)[:, :N]
+        half = torch.maximum((want.abs() + tol) * 2.0 ** -4, s * 2.0 ** -10)
+        assert ((r.data.double() * s - want).abs() <= half + tol).all()
+
+
 def test_one_block_at_a_time_takes_its_own_scale():
     """Every block of 128 holds ones in one place; the result is the product of the two scales of that block."""
     K, N, M = 128 * 5, 128 * 3, 160

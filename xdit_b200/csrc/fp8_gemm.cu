@@ -23,8 +23,8 @@
 // last ones are added, the buffer released before its last sums, arrivals without branches, the loop unrolled by
 // four (853 cycles without these).  Four warpgroups of 64 columns run out of registers (855).  Over seconds the power
 // limit sets the clock: 75,600 x 5120 x 15360 takes 5.57 ms (2.13 PFLOP/s) at about 1.4 GHz, a library product with one
-// scale for everything 4.5-4.6 ms; 9450 x 5120 x 13824 takes 629 us.  With few tiles it is the longest K axis of a CTA
-// that counts (273 x 6528 x 352: 9 tiles, 25.8 us).
+// scale for everything 4.5-4.6 ms; 9450 x 5120 x 13824 takes 629 us.  Few tiles of a long K axis go to the kernel for few rows,
+// which splits it.
 //
 // Every wait on an mbarrier is bounded in time; when one gives up the CTA raises a flag in shared memory, all
 // roles leave their loops, outstanding copies and MMAs are drained with bounded waits, TMEM is freed and
@@ -879,8 +879,18 @@ int configure_smem(int bytes) {
   return XDIT_OK;
 }
 
-// Few rows: NB the smallest of 16, 32, 64 that holds them (tiles of 64 above), the K axis split while two CTAs per SM
-// are not reached and a CTA keeps four steps.
+// CTAs that share the K axis of a tile when there are `tiles` of them: split in two up to three CTAs for two SMs, in four
+// up to one for each, in eight up to three quarters of that, while a CTA keeps four steps.  Two CTAs fit an SM, but a
+// cluster takes its places in one group of SMs, and what does not fit starts when others have ended (2 rows of 5120 to 4608:
+// 36 tiles by 8 13.3 us, by 4 9.5; 2 rows to 9216: 72 by 4 16.8, by 2 12.8; 64 rows to 2304: 18 by 8 15.8, by 4 11.8; 2 rows
+// of 13,824 to 1536: 12 by 8 9.8, by 4 12.1; 320 rows of 5120 to 2304: 90 by 2 20.2, whole 23.9).
+int rows_splits(int64_t tiles, int kb, int sms) {
+  int splits = 1;
+  while (splits < kMaxSplits && tiles * splits * 2 <= (splits == 1 ? sms + sms / 2 : splits == 2 ? sms : sms * 3 / 4) && kb / (splits * 2) >= 4) splits *= 2;
+  return splits;
+}
+
+// Few rows, or few tiles: NB the smallest of 16, 32, 64 that holds the rows, tiles of 64 above.
 template <int NB>
 int launch_rows(GemmArgs& a, const xdit_fp8_linear_params& p, int sms, bool after_quantise, cudaStream_t stream) {
   using L = RowsLayout<NB>;
@@ -889,8 +899,7 @@ int launch_rows(GemmArgs& a, const xdit_fp8_linear_params& p, int sms, bool afte
   if ((rc = encode_map(&a.tm_x, u8, 1, p.x, p.M, p.K, p.x_stride_row, NB, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   if ((rc = encode_map(&a.tm_w, u8, 1, p.w, p.N, p.K, p.w_stride_row, 128, kBK, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
   const int nt = (p.N + 127) / 128, mt = (p.M + NB - 1) / NB;
-  a.splits = 1;
-  while (a.splits < kMaxSplits && (int64_t)nt * mt * a.splits * 2 <= 2 * sms && a.kb / (a.splits * 2) >= 4) a.splits *= 2;
+  a.splits = rows_splits((int64_t)nt * mt, a.kb, sms);
   if ((rc = configure_smem<fp8_rows_kernel<NB>>(L::kSmem))) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(nt * a.splits), (unsigned)mt);
@@ -980,6 +989,12 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
     if (p->M <= 32) return launch_rows<32>(a, *p, sms, quantise, (cudaStream_t)stream);
     return launch_rows<64>(a, *p, sms, quantise, (cudaStream_t)stream);
   }
+  // Few tiles of a long K axis: here a tile's steps follow one another in one CTA (about 6.5 us + 0.42 us a step), there a
+  // cluster shares them (8.5 us + 0.55 us a step of a CTA).  It is worth it from two CTAs a tile and 16 steps on (65 rows of
+  // 4096 to 5120: 17.7 us split and 20.0 whole, of 13,824 38.5 and 56.0, 256 rows of 6528 to 352 11.8 and 27.1; below, 65
+  // rows of 1152 to 1152 10.0 and 8.7).
+  if (a.kb >= 16 && rows_splits((int64_t)((p->N + 127) / 128) * ((p->M + 63) / 64), a.kb, sms) > 1)
+    return launch_rows<64>(a, *p, sms, quantise, (cudaStream_t)stream);
   // Pairs of CTAs take tiles of 256 rows, single CTAs of 128.  A pair reads W once for twice the rows, but starts and
   // ends later and wastes more of a last, partly filled wave: it is worth it from four waves on (5120 x 5120: 2048
   // rows 58 us by pairs and 56 by single CTAs, 4096 rows 98 and 103, 18,900 rows 409 and 437).
