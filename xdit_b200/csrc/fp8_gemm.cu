@@ -215,6 +215,10 @@ __device__ __forceinline__ void report(const GemmArgs& a, volatile int* abort_fl
     }
   }
 }
+// A launch with quantising may start before the kernel that quantises x has ended.  Every CTA waits for that end, one that
+// skips its work too: what comes next on the stream is ordered behind this kernel alone, and may be given the memory that
+// the quantised rows are written to.
+__device__ __forceinline__ void wait_for_quantise() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Tile t: its row and column of tiles.
 __device__ __forceinline__ void tile_at(const GemmArgs& a, int t, int& m, int& n) {
   const int band = t / (a.band * a.nt), rem = t - band * a.band * a.nt;
@@ -280,12 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 
   if (skip) {
     // nothing to do: fall through to the teardown, which frees TMEM
+    wait_for_quantise();
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");  // per scheduler 2 x 232 + 40 = 3 x 168, what the launch holds
     if (warp == 9) {
       // ======================= TMA producer =======================
       if (lane == 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // a kernel that quantises x may still be running until here
+        wait_for_quantise();  // x is complete from here on
         int issued = 0;
         bool ok = a.selftest_stall == 0;
         for (int t = tile0; t < tiles && ok; t += tile_step) {
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     } else if (warp == 10) {
       // ======================= scales: each lane the rows lane, lane + 32, ... of the tile =======================
       // A load from L2 takes longer than a step, so they are copied asynchronously, up to kAhead steps ahead.
-      asm volatile("griddepcontrol.wait;" ::: "memory");
+      wait_for_quantise();
       int step = 0;
       bool ok = true;
       for (int t = tile0; t < tiles && ok; t += tile_step) {
@@ -629,6 +634,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
 
   if (skip) {
     // nothing to do: fall through to the teardown, which frees TMEM
+    wait_for_quantise();
   } else if (warp == 5) {
     // ======================= TMA producer =======================
     if (lane == 0) {
@@ -641,7 +647,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
       };
       const int first = a.selftest_stall ? 0 : min(steps, kStages);
       for (int i = 0; i < first; ++i) load_w(i);
-      asm volatile("griddepcontrol.wait;" ::: "memory");  // x is complete from here on
+      wait_for_quantise();  // x is complete from here on
       for (int i = 0; i < first; ++i) load_x(i);
       int issued = first;
       ok = a.selftest_stall == 0;
@@ -659,7 +665,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
     }
   } else if (warp == 6) {
     // ======================= scales =======================
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_quantise();
     constexpr int kPer = (NB + 31) / 32;
     const float* src[kPer];
 #pragma unroll
