@@ -563,8 +563,8 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
     set_error("%s: unknown norm %d or post_norm %d", who, p.norm, p.post_norm);
     return XDIT_E_DTYPE;
   }
+  if (p.B == 0 || p.s == 0) return XDIT_OK;  // (an empty tensor has no address: NULL does not mean absent here)
   if (p.norm == XDIT_NORM_NONE && !p.branch) { set_error("%s: nothing to do without a norm and a branch", who); return XDIT_E_SHAPE; }
-  if (p.B == 0 || p.s == 0) return XDIT_OK;
   if (!p.residual || (p.branch && !p.out_residual) || (p.norm != XDIT_NORM_NONE && !p.out && !p.out_q) ||
       (p.out_q && !p.out_scale)) {
     set_error("%s: NULL residual or output", who);

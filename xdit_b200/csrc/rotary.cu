@@ -243,7 +243,8 @@ __global__ void __launch_bounds__(kThreads) rotary_tables_kernel(const __grid_co
   *reinterpret_cast<float2*>(sin + row * a.D + 2 * pair) = make_float2(s, s);
 }
 
-int fill_positions(RotaryArgs& a, const xdit_rotary_positions& p, const char* who) {
+// Without `tokens` there may be no positions to point at.
+int fill_positions(RotaryArgs& a, const xdit_rotary_positions& p, bool tokens, const char* who) {
   if (p.pairs < 1 || p.pairs > XDIT_ROTARY_MAX_PAIRS || p.axes < 1 || p.axes > XDIT_ROTARY_MAX_AXES) {
     set_error("%s: %d pairs (1..%d) on %d axes (1..%d)", who, p.pairs, XDIT_ROTARY_MAX_PAIRS, p.axes, XDIT_ROTARY_MAX_AXES);
     return XDIT_E_SHAPE;
@@ -268,7 +269,7 @@ int fill_positions(RotaryArgs& a, const xdit_rotary_positions& p, const char* wh
     a.start = p.start;
     a.grid_small = volume < (1ll << 31) && p.start < (1ll << 31);  // start + row stays below 2^32
   } else {
-    if (!p.positions) { set_error("%s: NULL positions", who); return XDIT_E_NULL; }
+    if (!p.positions && tokens) { set_error("%s: NULL positions", who); return XDIT_E_NULL; }
     a.pos = p.positions;
     a.pos_sb = p.stride_b;
     a.pos_srow = p.stride_row;
@@ -290,7 +291,7 @@ cudaError_t launch(const RotaryArgs& a, bool halves, dim3 grid, cudaStream_t str
 int launch_rotary(const xdit_rotary_params& p, cudaStream_t stream) {
   RotaryArgs a;
   memset(&a, 0, sizeof(a));
-  int rc = fill_positions(a, p.pos, "xdit_rotary_axes");
+  int rc = fill_positions(a, p.pos, p.B > 0 && p.s > 0, "xdit_rotary_axes");
   if (rc) return rc;
   const int es = dtype_size(p.dtype);
   if (!es) { set_error("xdit_rotary_axes: bad dtype %d", p.dtype); return XDIT_E_DTYPE; }
@@ -377,7 +378,7 @@ int launch_rotary_tables(const xdit_rotary_positions& pos, float* cos, float* si
                          cudaStream_t stream) {
   RotaryArgs a;
   memset(&a, 0, sizeof(a));
-  int rc = fill_positions(a, pos, "xdit_rotary_tables");
+  int rc = fill_positions(a, pos, s > 0, "xdit_rotary_tables");
   if (rc) return rc;
   if (s < 0 || D < 2 || D % 2 || D > 4096 || a.rot > D) {
     set_error("xdit_rotary_tables: s=%d D=%d, %d elements rotated", s, D, a.rot);
