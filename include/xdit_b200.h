@@ -378,9 +378,11 @@ XDIT_API int xdit_rotary_tables(const struct xdit_rotary_positions* pos, float* 
  *   out_residual = residual_scale * residual + gate * post_norm(branch)     (without a branch: residual itself)
  *   out          = norm(...) * (1 + scale) + shift
  * with norms XDIT_NORM_NONE, _LAYER (mean and variance) or _RMS, each with an optional weight and bias.  norm
- * takes the unrounded sum.  Rows of modulation (xdit_row_vec, NULL ptr: absent) hold C contiguous values in
- * `dtype` or fp32; their strides are 0 where samples or tokens share a row.  post_weight, post_bias, weight
- * and bias are shared by all rows.  out_residual may be residual or branch itself.
+ * takes the unrounded sum; with XDIT_NORM_NONE there is no `out`, and out, out_q, weight, bias, scale and shift are
+ * NULL, as are post_weight and post_bias without a post_norm, and post_norm and gate without a branch.  Rows of
+ * modulation (xdit_row_vec, NULL ptr: absent) hold C contiguous values in `dtype` or fp32; their strides are 0
+ * where samples or tokens share a row.  post_weight, post_bias, weight and bias are shared by all rows.
+ * out_residual may be residual or branch itself.
  * With out_q the second result is written as e4m3 rows instead of `out`: [B*s, C] bytes and one scale
  * for each block of 128, out_scale[block * out_scale_ld + row]; needs C % 16 == 0 and 16-byte aligned rows.
  * Replaces: norm1/norm2 + modulation + gated residual around the attention and the MLP of the blocks that

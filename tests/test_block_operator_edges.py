@@ -21,10 +21,10 @@ PAIR = ctypes.c_int64 * 2
 
 
 def _rotary(lib, **kw):
-    """``xdit_rotary_axes`` on made-up addresses: what gets past the refusals ends at the missing device."""
+    """``xdit_rotary_axes`` on made-up addresses, one of them between two elements: no call gets past that refusal (-3)."""
     pos = dict(kind=0, axes=1, pairs=8, frequencies=F, axis=AXIS)
     pos.update({k[4:]: kw.pop(k) for k in list(kw) if k.startswith("pos_")})
-    p = _capi.RotaryParams(dtype=0, B=1, H=2, Hk=0, s=4, D=16, q=1 << 20, out_q=2 << 20, stride_h=PAIR(64, 64), stride_row=PAIR(16, 16),
+    p = _capi.RotaryParams(dtype=0, B=1, H=2, Hk=0, s=4, D=16, q=(1 << 20) + 1, out_q=2 << 20, stride_h=PAIR(64, 64), stride_row=PAIR(16, 16),
                            out_stride_h=PAIR(64, 64), out_stride_row=PAIR(16, 16), pos=_capi.RotaryPositions(**pos))
     p.pos.grid[0] = 4
     for k, v in kw.items():
@@ -33,7 +33,8 @@ def _rotary(lib, **kw):
 
 
 def _norm(lib, **kw):
-    p = _capi.NormParams(dtype=0, B=1, s=2, C=32, norm=1, residual=1 << 20, out=2 << 20, residual_stride_row=32, out_stride_row=32)
+    """``xdit_gated_residual_norm`` in the same way."""
+    p = _capi.NormParams(dtype=0, B=1, s=2, C=32, norm=1, residual=(1 << 20) + 1, out=2 << 20, residual_stride_row=32, out_stride_row=32)
     for k, v in kw.items():
         setattr(p, k, v)
     return lib.xdit_gated_residual_norm(ctypes.byref(p), None)
@@ -72,3 +73,38 @@ def test_no_tokens():
         assert h.shape == x.shape and z.shape == x.shape
     cos, sin = RotaryEmbedding((16, 16), positions=torch.empty(0, 2, dtype=torch.int32, device="cuda")).tables(0, 32, "cuda")
     assert cos.shape == sin.shape == (0, 32)
+
+
+# ---- parameters that nothing would read, results that nothing would write ---------------------------------------------
+BRANCH = dict(branch=3 << 20, branch_stride_row=32, out_residual=4 << 20, out_residual_stride_row=32)
+ROW = _capi.RowVec(ptr=5 << 20, dtype=0)
+
+
+def test_norm_c_entry_refuses_what_it_would_not_use(lib):
+    """Without a norm there is no second result to write, and no row that only the norm takes is read; the same holds for the
+    post norm and for the branch."""
+    past = -3  # the answer of a call that is refused for its address alone
+    assert _norm(lib, **BRANCH) == past
+    alone = {**BRANCH, "norm": 0, "out": None}
+    assert _norm(lib, **alone) == past
+    assert _norm(lib, **{**alone, "out": 2 << 20, "out_stride_row": 32}) == -2
+    assert _norm(lib, **alone, out_q=6 << 20, out_scale=7 << 20, out_scale_ld=2) == -2
+    for row in ("weight", "bias", "scale", "shift"):
+        assert _norm(lib, **alone, **{row: ROW}) == -2
+        assert _norm(lib, **BRANCH, **{row: ROW}) == past
+    for row in ("post_weight", "post_bias"):
+        assert _norm(lib, **BRANCH, **{row: ROW}) == -2
+        assert _norm(lib, **BRANCH, post_norm=2, **{row: ROW}) == past
+        assert _norm(lib, post_norm=2, **{row: ROW}) == -2
+    assert _norm(lib, gate=ROW) == -2 and _norm(lib, post_norm=1) == -2
+    assert _norm(lib, **BRANCH, gate=ROW) == past
+
+
+def test_ops_norm_refuses_a_second_result_without_a_norm():
+    from xdit_b200 import ops
+
+    x = torch.zeros(1, 3, 32)
+    q, s = ops.empty_fp8_rows(3, 32, "cpu")
+    for kw in (dict(out=torch.empty_like(x)), dict(out_q=q, out_scale=s)):
+        with pytest.raises(ValueError, match="norm"):
+            ops.gated_residual_norm(x, x.clone(), out_residual=torch.empty_like(x), **kw)

@@ -1,6 +1,6 @@
 // The steps of a DiT block between two sub-layers in one pass over a token's row:
 //   h = residual_scale * residual + gate * post(branch)      post: none, LayerNorm or RMSNorm
-//   z = norm(h) * (1 + scale) + shift                        norm: none, LayerNorm or RMSNorm
+//   z = norm(h) * (1 + scale) + shift                        norm: LayerNorm or RMSNorm (none: no z)
 // with h and z written, or z as e4m3 rows with one scale for each block of 128 (fp8_quant.cuh) where
 // an 8-bit projection follows.  gate, scale and shift hold one row for all tokens, for each sample, or
 // for each token.
@@ -565,6 +565,15 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
   }
   if (p.B == 0 || p.s == 0) return XDIT_OK;  // (an empty tensor has no address: NULL does not mean absent here)
   if (p.norm == XDIT_NORM_NONE && !p.branch) { set_error("%s: nothing to do without a norm and a branch", who); return XDIT_E_SHAPE; }
+  const bool post_rows = p.post_weight.ptr || p.post_bias.ptr, rows = p.weight.ptr || p.bias.ptr || p.scale.ptr || p.shift.ptr;
+  if (p.norm == XDIT_NORM_NONE && (p.out || p.out_q || rows)) {
+    set_error("%s: without a norm there is no second result, and weight, bias, scale and shift have nothing to apply to", who);
+    return XDIT_E_SHAPE;
+  }
+  if ((p.post_norm == XDIT_NORM_NONE && post_rows) || (!p.branch && (p.post_norm != XDIT_NORM_NONE || p.gate.ptr))) {
+    set_error("%s: post_weight and post_bias need a post norm; that and a gate need a branch", who);
+    return XDIT_E_SHAPE;
+  }
   if (!p.residual || (p.branch && !p.out_residual) || (p.norm != XDIT_NORM_NONE && !p.out && !p.out_q) ||
       (p.out_q && !p.out_scale)) {
     set_error("%s: NULL residual or output", who);

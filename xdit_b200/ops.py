@@ -752,8 +752,9 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], 
                         post_weight=None, post_bias=None, norm=None, weight=None, bias=None, scale=None, shift=None,
                         eps: float = 1e-6) -> None:
     """``out_residual = residual_scale * residual + gate * post_norm(branch)`` and ``out = norm(that) * (1 + scale) +
-    shift`` in one launch (``xdit_gated_residual_norm``); all ``[B, s, C]``.  ``out_q`` (e4m3 ``[B*s, C]``) with ``out_scale``
-    (fp32 ``[B*s, C/128]``, stored block by block) takes the second result quantised instead of ``out``."""
+    shift`` in one launch (``xdit_gated_residual_norm``); all ``[B, s, C]``.  Without a norm there is no ``out``.  ``out_q``
+    (e4m3 ``[B*s, C]``) with ``out_scale`` (fp32 ``[B*s, C/128]``, stored block by block) takes the second result quantised
+    instead of ``out``."""
     global launch_count
     if residual.dim() != 3:
         raise ValueError("expected [B, s, C]")
@@ -761,6 +762,8 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor], 
         raise ValueError("a norm is None, 'layer' or 'rms'")
     if norm is None and (weight is not None or bias is not None or scale is not None or shift is not None):
         raise ValueError("weight, bias, scale and shift need a norm")
+    if norm is None and (out is not None or out_q is not None):
+        raise ValueError("out and out_q need a norm")
     if branch is None and (post_norm is not None or gate is not None):
         raise ValueError("gate and post_norm need a branch")
     if post_norm is None and (post_weight is not None or post_bias is not None):
