@@ -108,3 +108,40 @@ def test_ops_norm_refuses_a_second_result_without_a_norm():
     for kw in (dict(out=torch.empty_like(x)), dict(out_q=q, out_scale=s)):
         with pytest.raises(ValueError, match="norm"):
             ops.gated_residual_norm(x, x.clone(), out_residual=torch.empty_like(x), **kw)
+
+
+# ---- outputs that lie on inputs ------------------------------------------------------------------------------------------
+def test_rotary_refuses_outputs_on_the_other_input_or_with_other_strides(lib):
+    """In place means each output in its own input, element by element: CTAs of q and of k run at the same time, and so do the
+    tokens of one."""
+    q, k, past = (1 << 20) + 1, 3 << 20, -3
+    both = dict(Hk=2, k=k, out_k=4 << 20)
+    assert _rotary(lib, **both) == past
+    assert _rotary(lib, **{**both, "out_k": k}) == past and _rotary(lib, out_q=q) == past  # in place
+    assert _rotary(lib, **{**both, "out_q": k}) == -2 and _rotary(lib, **{**both, "out_k": q}) == -2
+    assert _rotary(lib, **{**both, "out_q": k, "out_k": q}) == -2
+    for strides in (dict(out_stride_row=PAIR(32, 16)), dict(out_stride_h=PAIR(128, 64)), dict(B=2, out_stride_b=PAIR(256, 256), stride_b=PAIR(128, 128))):
+        assert _rotary(lib, out_q=q, **strides) == -2 and _rotary(lib, **strides) == past
+    for strides in (dict(out_stride_row=PAIR(16, 32)), dict(out_stride_h=PAIR(64, 128))):
+        assert _rotary(lib, **{**both, "out_k": k}, **strides) == -2 and _rotary(lib, **both, **strides) == past
+    # a stride that no step takes may be any
+    assert _rotary(lib, out_q=q, s=1, out_stride_row=PAIR(32, 16)) == past and _rotary(lib, out_q=q, H=1, out_stride_h=PAIR(1, 1)) == past
+
+
+@pytest.mark.gpu
+def test_rotary_in_place_and_in_refused_places():
+    from xdit_b200._capi import XditError
+    from xdit_b200.rotary import RotaryEmbedding, rotary_embed
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k = (torch.randn(2, 3, 40, 32, device="cuda", generator=g) for _ in range(2))
+    e = RotaryEmbedding((16, 16), grid=(5, 8))
+    a, b = rotary_embed(q, k, e)
+    kept = q.clone(), k.clone()
+    with pytest.raises(XditError):
+        rotary_embed(q, k, e, out_query=k, out_key=q)
+    with pytest.raises(XditError):
+        rotary_embed(q, q, e, out_query=q, out_key=k)
+    assert torch.equal(q, kept[0]) and torch.equal(k, kept[1])
+    rotary_embed(q, k, e, out_query=q, out_key=k)
+    assert torch.equal(q, a) and torch.equal(k, b)

@@ -322,6 +322,13 @@ int launch_rotary(const xdit_rotary_params& p, cudaStream_t stream) {
       return XDIT_E_SHAPE;
     }
   if (p.Hk && p.out_q == p.out_k) { set_error("xdit_rotary_axes: q and k have one output"); return XDIT_E_SHAPE; }
+  if (p.Hk && (p.out_q == p.k || p.out_k == p.q)) { set_error("xdit_rotary_axes: an output lies on the other input"); return XDIT_E_SHAPE; }
+  for (int t = 0; t < (p.Hk ? 2 : 1); ++t)
+    if (a.src[t] == a.dst[t] && ((p.B > 1 && a.ss_b[t] != a.ds_b[t]) || (a.heads[t] > 1 && a.ss_h[t] != a.ds_h[t]) ||
+                                 (p.s > 1 && a.ss_row[t] != a.ds_row[t]))) {
+      set_error("xdit_rotary_axes: an output lies on its input with other strides");
+      return XDIT_E_SHAPE;
+    }
   if (low % es) { set_error("xdit_rotary_axes: a pointer is not aligned to its elements"); return XDIT_E_ALIGN; }
   int sms = 0;
   if ((rc = check_device(&sms))) return rc;

@@ -89,8 +89,8 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], embedding: Ro
                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(query, key)`` rotated by ``embedding``.  ``query`` ``[B, H, s, D]`` and ``key`` ``[B, Hk, s, D]`` (or ``None``; its heads may be
     fewer) in bf16, fp16 or fp32, any strides with a contiguous last axis.  The results lie in memory like the inputs, or
-    go to ``out_query`` / ``out_key``, which may be the inputs themselves.  Angles are taken in 64 bits and their cos and
-    sin in 32; a result is rounded once."""
+    go to ``out_query`` / ``out_key``, which may be the inputs themselves (each its own) but not overlap them in another
+    way.  Angles are taken in 64 bits and their cos and sin in 32; a result is rounded once."""
     if torch.compiler.is_compiling() and out_query is None and out_key is None:
         from . import compile_ops
 
