@@ -382,7 +382,7 @@ XDIT_API int xdit_rotary_tables(const struct xdit_rotary_positions* pos, float* 
  * NULL, as are post_weight and post_bias without a post_norm, and post_norm and gate without a branch.  Rows of
  * modulation (xdit_row_vec, NULL ptr: absent) hold C contiguous values in `dtype` or fp32; their strides are 0
  * where samples or tokens share a row.  post_weight, post_bias, weight and bias are shared by all rows.
- * out_residual may be residual or branch itself.
+ * out_residual may be residual or branch itself (same strides); no output may overlap an input in another way.
  * With out_q the second result is written as e4m3 rows instead of `out`: [B*s, C] bytes and one scale
  * for each block of 128, out_scale[block * out_scale_ld + row]; needs C % 16 == 0 and 16-byte aligned rows.
  * Replaces: norm1/norm2 + modulation + gated residual around the attention and the MLP of the blocks that

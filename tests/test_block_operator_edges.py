@@ -145,3 +145,36 @@ def test_rotary_in_place_and_in_refused_places():
     assert torch.equal(q, kept[0]) and torch.equal(k, kept[1])
     rotary_embed(q, k, e, out_query=q, out_key=k)
     assert torch.equal(q, a) and torch.equal(k, b)
+
+
+def test_norm_refuses_outputs_on_the_modulation_or_with_other_strides(lib):
+    past, x = -3, (1 << 20) + 1
+    h = dict(BRANCH)
+    assert _norm(lib, **{**h, "out_residual": x}) == past and _norm(lib, **{**h, "out_residual": h["branch"]}) == past  # in place
+    assert _norm(lib, out=x) == past
+    for at in (x, h["branch"]):
+        assert _norm(lib, **{**h, "out_residual": at, "out_residual_stride_row": 64}) == -2
+        assert _norm(lib, **{**h, "out": at, "out_stride_row": 64}) == -2
+        far = dict(B=2, residual_stride_b=64, branch_stride_b=64, out_residual_stride_b=128, out_stride_b=128)
+        assert _norm(lib, **{**h, **far, "out_residual": at}) == -2 and _norm(lib, **{**h, **far, "out": at}) == -2
+        assert _norm(lib, **{**h, "s": 1, "out_residual": at, "out_residual_stride_row": 64}) == past
+    for row in ("gate", "weight", "bias", "scale", "shift", "post_weight", "post_bias"):
+        rows = {**h, "post_norm": 1, row: ROW}
+        assert _norm(lib, **rows) == past
+        assert _norm(lib, **{**rows, "out_residual": ROW.ptr}) == -2 and _norm(lib, **rows, out=ROW.ptr) == -2
+
+
+@pytest.mark.gpu
+def test_norm_in_place_and_in_refused_places():
+    from xdit_b200._capi import XditError
+    from xdit_b200.modulation import gated_residual_norm
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, y, gate = (torch.randn(2, 5, 64, device="cuda", generator=g) for _ in range(3))
+    h, z = gated_residual_norm(x, y, gate=gate)
+    with pytest.raises(XditError):
+        gated_residual_norm(x, y, gate=gate, out_residual=gate)
+    for which in (0, 1):
+        both = [x.clone(), y.clone()]
+        h1, z1 = gated_residual_norm(*both, gate=gate, out_residual=both[which])
+        assert h1 is both[which] and torch.equal(h1, h) and torch.equal(z1, z)

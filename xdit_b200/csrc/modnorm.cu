@@ -609,13 +609,31 @@ int launch_norm(const xdit_norm_params& p, cudaStream_t stream) {
     to[i]->f32 = in[i]->dtype != XDIT_F32 ? 0 : apart ? 1 : 2;
     look(in[i]->ptr, in[i]->stride_b, in[i]->stride_row, dtype_size(in[i]->dtype));
   }
-  if (off) { set_error("%s: a pointer is not aligned to its elements", who); return XDIT_E_ALIGN; }
   const bool h_one = p.out_residual && ((p.B > 1 && !p.out_residual_stride_b) || (p.s > 1 && !p.out_residual_stride_row));
   const bool z_one = p.out && !p.out_q && ((p.B > 1 && !p.out_stride_b) || (p.s > 1 && !p.out_stride_row));
   if (h_one || z_one || (p.norm != XDIT_NORM_NONE && p.out && p.out == p.out_residual)) {
     set_error("%s: an output holds several rows in one place, or both outputs are one", who);
     return XDIT_E_SHAPE;
   }
+  // In place: element by element in residual or branch.  Rows are read while others are written, so an output at the
+  // address of either with other strides, or on a row of modulation, would be read as it changes.
+  bool torn = false;
+  auto place = [&](const void* o, int64_t sb, int64_t srow) {
+    if (!o) return;
+    auto on = [&](const void* x, int64_t xb, int64_t xrow) {
+      torn |= o == x && ((p.B > 1 && sb != xb) || (p.s > 1 && srow != xrow));
+    };
+    on(p.residual, p.residual_stride_b, p.residual_stride_row);
+    on(p.branch, p.branch_stride_b, p.branch_stride_row);
+    for (const xdit_row_vec* v : in) torn |= o == v->ptr;
+  };
+  place(p.out_residual, p.out_residual_stride_b, p.out_residual_stride_row);
+  if (!p.out_q) place(p.out, p.out_stride_b, p.out_stride_row);
+  if (torn) {
+    set_error("%s: an output lies on residual or branch with other strides, or on a row of modulation", who);
+    return XDIT_E_SHAPE;
+  }
+  if (off) { set_error("%s: a pointer is not aligned to its elements", who); return XDIT_E_ALIGN; }
   const bool wide = p.C % 8 == 0 && (low & 15) == 0;
   if (!wide)
     for (RowVec* v : to) v->f32 = v->f32 != 0;  // 32 bytes are the width of V = 8
