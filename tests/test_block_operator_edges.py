@@ -178,3 +178,25 @@ def test_norm_in_place_and_in_refused_places():
         both = [x.clone(), y.clone()]
         h1, z1 = gated_residual_norm(*both, gate=gate, out_residual=both[which])
         assert h1 is both[which] and torch.equal(h1, h) and torch.equal(z1, z)
+
+
+# ---- positions of the tables that the attention prologue takes ------------------------------------------------------------
+def test_tables_look_at_their_positions(monkeypatch):
+    """The kernel that rotates runs on the query's device and reads the tables there."""
+    from xdit_b200 import ops
+    from xdit_b200.rotary import RotaryEmbedding
+
+    e = RotaryEmbedding((8, 8), positions=torch.zeros(5, 2))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        e.tables(5, 16, "cuda")
+    with pytest.raises(NotImplementedError, match="backward"):
+        RotaryEmbedding((8, 8), positions=torch.zeros(5, 2, requires_grad=True)).tables(5, 16, "cuda")
+    made = []
+    monkeypatch.setattr(ops, "_check_tensors", lambda *t: None)  # (as if the positions were on a GPU)
+    monkeypatch.setattr(ops, "rotary_tables", lambda p, s, D, device: made.append(device) or (None, None))
+    with pytest.raises(ValueError, match="cuda:1"):
+        e.tables(5, 16, "cuda:1")
+    with pytest.raises(ValueError):
+        e.tables(5, 16, torch.device("cuda", 0))
+    e.tables(5, 16, "cpu")
+    assert made == [torch.device("cpu")]

@@ -79,8 +79,11 @@ class RotaryEmbedding:
         if D < sum(self.axes_dim):
             raise ValueError(f"{sum(self.axes_dim)} elements to rotate in a head of {D}")
         if self.positions is not None:
-            ops._require_cuda(self.positions)
-            device = self.positions.device
+            ops._check_tensors(self.positions)
+            device, at = torch.device(device), self.positions.device
+            if device.type != at.type or device.index not in (None, at.index):
+                raise ValueError(f"positions on {at} and tables on {device}")
+            device = at
         return ops.rotary_tables(self._params(1, s), s, D, device)
 
 
