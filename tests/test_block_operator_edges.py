@@ -200,3 +200,41 @@ def test_tables_look_at_their_positions(monkeypatch):
         e.tables(5, 16, torch.device("cuda", 0))
     e.tables(5, 16, "cpu")
     assert made == [torch.device("cpu")]
+
+
+# ---- an embedding that does not fit, beside a stale-KV buffer ------------------------------------------------------------
+@pytest.mark.parametrize("pairing", ["interleaved", "halves"])
+@pytest.mark.parametrize("wrong", ["tokens", "head", "type", "pairing", "gradient"])
+def test_a_refused_embedding_leaves_the_stale_buffers_alone(monkeypatch, pairing, wrong):
+    """Keys that have been written but not rotated would be what the next steps attend to.  Interleaved pairs are rotated by
+    tables in the prologue, halves behind it."""
+    import xdit_b200
+    from tests import fake_ops
+    from xdit_b200 import cache_manager, ops
+    from xdit_b200.prologue import attention_from_projections
+    from xdit_b200.rotary import RotaryEmbedding
+
+    def check(*tensors):  # (as on a GPU)
+        if any(t.requires_grad for t in tensors):
+            raise NotImplementedError
+
+    fake_ops.install(monkeypatch)
+    monkeypatch.setattr(ops, "_check_tensors", check)
+    xdit_b200.init_sequence_parallel(1, 1)
+    manager = cache_manager.CacheManager()
+    manager.register_cache_entry("layer", "attn")
+    monkeypatch.setattr(cache_manager, "get_cache_manager", lambda: manager)
+    monkeypatch.setattr(cache_manager, "runtime_state_is_initialized", lambda: False)
+    B, n, H, D = 2, 6, 2, 16
+    entry = manager.cache["attn", "layer"]
+    entry.k, entry.v = torch.ones(B, H, n + 2, D), torch.ones(B, H, n + 2, D)
+    k, v = entry.k, entry.v
+    ids = torch.zeros(n, 2) if pairing == "interleaved" else torch.zeros(B, n, 2)
+    kw = dict(axes_dim=(8, 8), positions=ids, pairing=pairing)
+    kw.update({"tokens": dict(positions=ids[..., 1:, :]), "head": dict(axes_dim=(12, 12)), "type": dict(positions=ids.double()),
+               "pairing": dict(pairing="thirds"), "gradient": dict(positions=ids.clone().requires_grad_())}[wrong])
+    x = torch.randn(B, n, H * D)
+    error = {"type": TypeError, "gradient": NotImplementedError}.get(wrong, ValueError)
+    with pytest.raises(error):
+        attention_from_projections(x, x, x, H, rotary_emb=RotaryEmbedding(**kw), attn_layer="layer")
+    assert entry.k is k and entry.v is v and (k == 1).all() and (v == 1).all()

@@ -61,6 +61,7 @@ def _rotary(rotary_emb, B, s, D, device):
     if isinstance(rotary_emb, RotaryEmbedding):
         p = rotary_emb.positions
         if rotary_emb.pairing != "interleaved" or (B > 1 and p is not None and p.dim() == 3 and p.shape[0] > 1):
+            rotary_emb._fit(B, s, D, device)  # what does not fit is refused before anything is written
             return None, None, rotary_emb
         return (*rotary_emb.tables(s, D, device), None)
     return (*_cos_sin(rotary_emb, s, D), None)
@@ -149,9 +150,9 @@ def _attention_with_stale_kv(query, key, value, heads, norm_q_weight, norm_k_wei
                                   "use USP(..., attn_layer=...) otherwise")
     B, n, HD = query.shape
     D = HD // heads
+    cos, sin, late = _rotary(rotary_emb, B, n, D, query.device)
     kc, vc, start = get_cache_manager().rows_for_producer(attn_layer, B, heads, n, D, query.dtype, query.device)
     S = kc.shape[2]
-    cos, sin, late = _rotary(rotary_emb, B, n, D, query.device)
     q_buf = torch.empty(heads * B * n * D, dtype=query.dtype, device=query.device)
     # q in the packed [H][B][n][D] layout; k and v rows at [start, start + n) of the [B,H,S,D] buffers
     ops.qk_norm_rope_pack(query, key, value, heads, q_buf, kc.view(-1)[start * D:], vc.view(-1)[start * D:],

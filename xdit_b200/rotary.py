@@ -71,20 +71,26 @@ class RotaryEmbedding:
         return ops.rotary_positions(freq, axis, pairs, len(self.axes_dim), positions=self.positions, grid=self.grid,
                                     start=self.start, batch=batch, rows=rows)
 
+    def _fit(self, batch: int, rows: int, D: int, device) -> Tuple[_capi.RotaryPositions, torch.device]:
+        """``(positions, device)`` for ``rows`` tokens of heads of ``D`` on ``device``, or the refusal that a launch would meet."""
+        device = torch.device(device)
+        if D < sum(self.axes_dim):
+            raise ValueError(f"{sum(self.axes_dim)} elements to rotate in a head of {D}")
+        if self.positions is not None:
+            ops._check_tensors(self.positions)
+            at = self.positions.device
+            if device.type != at.type or device.index not in (None, at.index):
+                raise ValueError(f"positions on {at} for tensors on {device}")
+            device = at
+        return self._params(batch, rows), device
+
     def tables(self, s: int, D: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
         """``(cos, sin)``, fp32 ``[s, D]``, as the attention prologue takes them: interleaved pairs, one set of positions for
         all samples."""
         if self.pairing != "interleaved":
             raise ValueError("the attention prologue rotates interleaved pairs")
-        if D < sum(self.axes_dim):
-            raise ValueError(f"{sum(self.axes_dim)} elements to rotate in a head of {D}")
-        if self.positions is not None:
-            ops._check_tensors(self.positions)
-            device, at = torch.device(device), self.positions.device
-            if device.type != at.type or device.index not in (None, at.index):
-                raise ValueError(f"positions on {at} and tables on {device}")
-            device = at
-        return ops.rotary_tables(self._params(1, s), s, D, device)
+        positions, device = self._fit(1, s, D, device)
+        return ops.rotary_tables(positions, s, D, device)
 
 
 def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], embedding: RotaryEmbedding, *,
