@@ -238,3 +238,25 @@ def test_a_refused_embedding_leaves_the_stale_buffers_alone(monkeypatch, pairing
     with pytest.raises(error):
         attention_from_projections(x, x, x, H, rotary_emb=RotaryEmbedding(**kw), attn_layer="layer")
     assert entry.k is k and entry.v is v and (k == 1).all() and (v == 1).all()
+
+
+# ---- gradients ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["hidden_states", "qkv_weight", "qkv_bias", "out_proj_weight", "out_proj_bias", "norm_q_weight"])
+def test_attention_from_hidden_states_refuses_a_gradient(monkeypatch, which):
+    """With 16- and 32-bit weights too: the projections would record it, and the attention between them would cut it."""
+    import xdit_b200
+    from tests import fake_ops
+    from xdit_b200.prologue import attention_from_hidden_states
+
+    fake_ops.install(monkeypatch)
+    xdit_b200.init_sequence_parallel(1, 1)
+    H, C = 2, 32
+    kw = dict(hidden_states=torch.randn(1, 5, C), qkv_weight=torch.randn(3 * C, C), qkv_bias=torch.randn(3 * C),
+              out_proj_weight=torch.randn(C, C), out_proj_bias=torch.randn(C), norm_q_weight=torch.ones(C),
+              norm_k_weight=torch.ones(C))
+    want = attention_from_hidden_states(heads=H, **kw)
+    kw[which].requires_grad_()
+    with pytest.raises(NotImplementedError, match="backward"):
+        attention_from_hidden_states(heads=H, **kw)
+    with torch.no_grad():
+        assert torch.equal(attention_from_hidden_states(heads=H, **kw), want)

@@ -581,11 +581,16 @@ def qk_norm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: 
     launch_count += 1
 
 
-def _check_tensors(first: torch.Tensor, *others) -> None:
-    """What every launch asks of its tensors: no gradient to record, CUDA memory, one device."""
-    if torch.is_grad_enabled() and (first.requires_grad or [t for t in others if t is not None and t.requires_grad]):
+def _refuse_gradient(*tensors) -> None:
+    """No gradient of ``tensors`` is to be recorded: a launch would cut it from its graph."""
+    if torch.is_grad_enabled() and [t for t in tensors if t is not None and t.requires_grad]:
         raise NotImplementedError("backward passes are not part of this inference path: call it under "
                                   "torch.no_grad(), or with tensors that do not require a gradient")
+
+
+def _check_tensors(first: torch.Tensor, *others) -> None:
+    """What every launch asks of its tensors: no gradient to record, CUDA memory, one device."""
+    _refuse_gradient(first, *others)
     if not first.is_cuda:
         _require_cuda(first)
     device = first.get_device()

@@ -127,7 +127,9 @@ def attention_from_hidden_states(hidden_states: Union[torch.Tensor, Fp8Rows], qk
     ``qkv_weight`` ``[3 * heads*D, hidden]``, :func:`attention_from_projections` with ``kwargs`` on its three column slices, and the
     output projection where one is given.  A weight may be an :class:`~xdit_b200.fp8_linear.Fp8Weight`; ``hidden_states`` may then
     be the :class:`~xdit_b200.fp8_linear.Fp8Rows` that ``gated_residual_norm(quantize=True)`` makes, and ``dtype`` is the type that
-    the attention runs in."""
+    the attention runs in.  Forward only: tensors that record a gradient are refused."""
+    given = (hidden_states, qkv_weight, qkv_bias, out_proj_weight, out_proj_bias, *kwargs.values())
+    ops._refuse_gradient(*(t for t in given if isinstance(t, torch.Tensor)))
     if isinstance(hidden_states, Fp8Rows):
         if not isinstance(qkv_weight, Fp8Weight):
             raise TypeError("e4m3 hidden states need an Fp8Weight as qkv_weight")
