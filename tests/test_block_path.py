@@ -271,3 +271,35 @@ def test_a_compiled_block_has_no_graph_break():
         dynamo.reset()
         got = torch.compile(block, fullgraph=True, backend="aot_eager")(x)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_captured_blocks_replay_to_the_bits_of_the_eager_ones():
+    """Two graphs of two blocks each, the second with positions of each sample's own, replayed in turn on changed inputs with
+    eager calls between."""
+    import xdit_b200
+    from xdit_b200 import ops
+    from xdit_b200.graph import GraphedStep
+    from xdit_b200.rotary import RotaryEmbedding
+
+    xdit_b200.init_sequence_parallel(1, 1)
+    B, grid, C_, heads = 2, (2, 9, 11), 512, 4
+    s, g = math.prod(grid), torch.Generator(device="cuda").manual_seed(7)
+    blocks = [_Block(C_, heads, 1280, seed) for seed in (8, 9)]
+    x = torch.randn(B, s, C_, device="cuda", generator=g).bfloat16()
+    ids = torch.randint(0, 60, (B, s, 3), device="cuda", generator=g)
+    embeddings = [RotaryEmbedding((48, 40, 40), grid=grid), RotaryEmbedding((48, 40, 40), positions=ids, ladder="shared")]
+
+    def two(e):
+        return blocks[1](blocks[0](x, e), e)
+
+    with torch.no_grad():
+        steps = [GraphedStep(lambda e=e: two(e)) for e in embeddings]
+        for _ in range(3):
+            x.copy_(torch.randn(B, s, C_, device="cuda", generator=g))
+            ids.copy_(torch.randint(0, 60, (B, s, 3), device="cuda", generator=g))
+            want = [two(e) for e in embeddings]
+            for step, w in ((steps[1], want[1]), (steps[0], want[0]), (steps[1], want[1])):
+                assert torch.equal(step.replay(), w)
+        torch.cuda.synchronize()
+        ops.check_status()
