@@ -260,3 +260,26 @@ def test_attention_from_hidden_states_refuses_a_gradient(monkeypatch, which):
         attention_from_hidden_states(heads=H, **kw)
     with torch.no_grad():
         assert torch.equal(attention_from_hidden_states(heads=H, **kw), want)
+
+
+# ---- the norm's kernels -------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [256 * i + d for i in (1, 2, 3, 4, 5) for d in (-8, 0, 8)] + [1024 * i + d for i in (2, 3, 4, 5) for d in (-8, 0, 8)]
+                         + [8192, 8200, 12288, 12296, 16376])
+def test_norm_at_both_ends_of_every_width_of_vectors(C):
+    """Rows of 16-byte words at the ends of every number of vectors a thread, both results against 64 bits.  Tolerance: a sum
+    of C values in a tree is off by less than 2^-24 (log2(C) + 40) of its magnitudes, the norm's other steps by ten roundings:
+    128 of 2^-24 of the magnitudes of what a value is made of, and half a spacing of bf16."""
+    from xdit_b200.modulation import gated_residual_norm
+
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x, y = (torch.randn(1, 3, C, device="cuda", generator=g).bfloat16() for _ in range(2))
+    gate, scale = (torch.randn(1, 1, C, device="cuda", generator=g) for _ in range(2))
+    h, z = gated_residual_norm(x, y, gate=gate, scale=scale, norm="rms")
+    wh = x.double() + gate.double() * y.double()
+    r = 1 / torch.sqrt((wh * wh).mean(-1, keepdim=True) + 1e-6)
+    wz = wh * r * (1 + scale.double())
+    mag = x.double().abs() + (gate.double() * y.double()).abs()
+    zmag = (mag * r + wh.abs() * r * (mag * mag).mean(-1, keepdim=True) * r * r) * (1 + scale.double().abs())
+    for got, want, m in ((h, wh, mag), (z, wz, zmag)):
+        assert ((got.double() - want).abs() <= 128 * 2.0 ** -24 * m + want.abs() * 2.0 ** -8).all()

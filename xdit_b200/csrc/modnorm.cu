@@ -509,20 +509,20 @@ cudaError_t launch(const NormArgs& a, int sms, cudaStream_t stream) {
 // 16 with the last ones idle; 3063 of 1155 by values 15.6 us by 10 a thread and 17.9 by 12.
 template <typename T>
 cudaError_t dispatch(const NormArgs& a, int V, int sms, cudaStream_t stream) {
-#define XDIT_VPT5(V, TPR)                                       \
-  switch ((a.nvec + TPR - 1) / TPR) {                           \
-    case 1: return launch<T, V, TPR, 1>(a, sms, stream);        \
-    case 2: return launch<T, V, TPR, 2>(a, sms, stream);        \
-    case 3: return launch<T, V, TPR, 3>(a, sms, stream);        \
-    case 4: return launch<T, V, TPR, 4>(a, sms, stream);        \
-    default: return launch<T, V, TPR, 5>(a, sms, stream);       \
-  }
   if (V == 8) {
-    if (a.nvec <= 160) XDIT_VPT5(8, 32)
-    if (a.nvec <= 640) XDIT_VPT5(8, 128)
-    XDIT_VPT5(8, 512)
+    if (a.nvec <= 32) return launch<T, 8, 32, 1>(a, sms, stream);
+    if (a.nvec <= 64) return launch<T, 8, 32, 2>(a, sms, stream);
+    if (a.nvec <= 96) return launch<T, 8, 32, 3>(a, sms, stream);
+    if (a.nvec <= 128) return launch<T, 8, 32, 4>(a, sms, stream);
+    if (a.nvec <= 160) return launch<T, 8, 32, 5>(a, sms, stream);
+    if (a.nvec <= 256) return launch<T, 8, 128, 2>(a, sms, stream);
+    if (a.nvec <= 384) return launch<T, 8, 128, 3>(a, sms, stream);
+    if (a.nvec <= 512) return launch<T, 8, 128, 4>(a, sms, stream);
+    if (a.nvec <= 640) return launch<T, 8, 128, 5>(a, sms, stream);
+    if (a.nvec <= 1024) return launch<T, 8, 512, 2>(a, sms, stream);
+    if (a.nvec <= 1536) return launch<T, 8, 512, 3>(a, sms, stream);
+    return launch<T, 8, 512, 4>(a, sms, stream);  // up to XDIT_NORM_MAX_C values
   }
-#undef XDIT_VPT5
   if (V == 2) {
     if (a.nvec <= 64) return launch<T, 2, 32, 2>(a, sms, stream);
     if (a.nvec <= 160) return launch<T, 2, 32, 5>(a, sms, stream);
