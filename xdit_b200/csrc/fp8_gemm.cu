@@ -314,11 +314,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             ++issued;
           }
         }
-        if constexpr (PAIR) {
-          // the MMAs report the last stages' release to both CTAs: neither may leave before that has arrived
-          for (int i = issued > kStages ? issued - kStages : 0; i < issued && ok; ++i)
-            ok = mbar_wait(bar_empty(i % kStages), (i / kStages) & 1, abort_flag, a.wait_limit_ns, 110);
-        }
+        // the MMAs report the last stages' release (of a pair, to both CTAs): none may leave before that has arrived
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued && ok; ++i)
+          ok = mbar_wait(bar_empty(i % kStages), (i / kStages) & 1, abort_flag, a.wait_limit_ns, 110);
         if (!ok) {
           // drain: every armed stage must have received its bytes before the CTA may leave (a pair: before either leaves)
           // (the second CTA's bytes count on the first one's barriers, which it cannot watch: it leaves them a thousand times
@@ -657,6 +655,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) fp8_rows_kernel(const __grid_
         load_w(issued);
         load_x(issued);
       }
+      // the MMAs report the last stages' release: the CTA may not leave before that has arrived
+      for (int i = issued > kStages ? issued - kStages : 0; i < issued && ok; ++i)
+        ok = mbar_wait(bar_empty(i % kStages), (i / kStages) & 1, abort_flag, a.wait_limit_ns, 110);
       if (!ok) {
         // drain: every armed stage must have received its bytes before the CTA may leave
         for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
