@@ -375,7 +375,7 @@ XDIT_API int xdit_rotary_tables(const struct xdit_rotary_positions* pos, float* 
                                 int32_t D, void* stream);
 
 /* The steps of a DiT block between two sub-layers, in one pass over each token's row of C values:
- *   out_residual = residual_scale * residual + gate * post_norm(branch)     (without a branch: residual itself)
+ *   out_residual = residual_scale * residual + gate * post_norm(branch)     (without a branch: residual, unscaled)
  *   out          = norm(...) * (1 + scale) + shift
  * with norms XDIT_NORM_NONE, _LAYER (mean and variance) or _RMS, each with an optional weight and bias.  norm
  * takes the unrounded sum; with XDIT_NORM_NONE there is no `out`, and out, out_q, weight, bias, scale and shift are
@@ -420,7 +420,7 @@ XDIT_API int xdit_quantize_weight(const void* w, int64_t stride_row, int32_t dty
                                   float* scale, void* stream);
 
 /* out[m, n] = act(sum_c x_scale[m, c] w_scale[n/128, c] sum_{k in block c} x[m, k] w[n, k] + bias[n]) with x
- * [M, K] and w [N, K] in e4m3 and scales of any value.  out: bf16, fp16 or fp32, rounded once; or, with
+ * [M, K] and w [N, K] in e4m3 and scales of any value whose products are within fp32's range.  out: bf16, fp16 or fp32, rounded once; or, with
  * out_q, e4m3 rows [M, N] with out_scale[block * out_scale_ld + row] (N % 16 == 0).  K % 16 == 0; rows of x and
  * w start on 16-byte boundaries.  status, status_host and wait_limit_ns as in xdit_attn_params.
  * Replaces: the fp8 linear layers of xfuser/model_executor/layers/fp8_linear.py. */

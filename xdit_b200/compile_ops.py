@@ -7,8 +7,8 @@ the ctypes calls (the reference wraps its own non-traceable kernels the same way
 * ``xdit_b200::usp``   -- a whole ``USP`` call under the current sequence-parallel state (pack, collectives,
   attention, return exchange), ``(q, k, v[, joint q, k, v]) -> out``.
 
-* ``xdit_b200::rotary_axes``, ``xdit_b200::gated_residual_norm`` (and ``_fp8``), ``xdit_b200::fp8_linear`` (and ``_fp8``) -- the
-  steps of a block around its attention; ``_fp8`` returns e4m3 rows and their scales.
+* ``xdit_b200::rotary_axes``, ``xdit_b200::gated_residual_norm``, ``xdit_b200::fp8_linear`` -- the steps of a block around its
+  attention, each a list of what the step makes (e4m3 rows as two tensors, values and scales).
 
 All are functional (they allocate their results) and carry shape-only "fake" implementations for
 tracing.  ``xdit_b200.USP``, the ``[B,S,H,D]`` layer and the block's functions route through them while Dynamo is

@@ -18,13 +18,14 @@
 // the whole time).  Or they become e4m3 rows again: a thread holds a whole block of its row.
 //
 // What bounds it: the MMAs alone take 533 cycles a step by pairs (595 by single CTAs; 512 is the tensor core's rate), the
-// scaled sums bring that to about 700.  They are 256 cycles of packed FMAs and the TMEM reads of two warps a scheduler,
-// and what counted was keeping the rest out of their way: scales copied ahead, the next 16 columns loaded while the
+// scaled sums bring that to about 700, and the tensor core waits for a tile's epilogue, which the summing warps do too: 4.5
+// us a tile, 6.8 with GELU (9472 x K to 9728 over K: 0.41 us a step beside that).  The sums are 256 cycles of packed FMAs and
+// the TMEM reads of two warps a scheduler, and what counted was keeping the rest out of their way: scales copied ahead, the next 16 columns loaded while the
 // last ones are added, the buffer released before its last sums, arrivals without branches, the loop unrolled by
 // four (853 cycles without these).  Four warpgroups of 64 columns run out of registers (855).  Over seconds the power
-// limit sets the clock: 75,600 x 5120 x 15360 takes 5.57 ms (2.13 PFLOP/s) at about 1.4 GHz, a library product with one
-// scale for everything 4.5-4.6 ms; 9450 x 5120 x 13824 takes 629 us.  Few tiles of a long K axis go to the kernel for few rows,
-// which splits it.
+// limit sets the clock: 75,600 x 5120 x 15360 takes 5.57-5.73 ms (2.07-2.13 PFLOP/s) at about 1.4 GHz, a library product with
+// one scale for everything 4.5-4.6 ms; 9450 x 5120 x 13824 takes 574-630 us (results in fp32 855, 16-bit ones off 16-byte
+// words 1706: they leave lane by lane).  Few tiles of a long K axis go to the kernel for few rows, which splits it.
 //
 // Every wait on an mbarrier is bounded in time; when one gives up the CTA raises a flag in shared memory, all
 // roles leave their loops, outstanding copies and MMAs are drained with bounded waits, TMEM is freed and

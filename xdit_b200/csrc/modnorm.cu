@@ -8,9 +8,9 @@
 // HBM-bound: residual and branch are read once, h and z written once; the row stays in registers (fp32,
 // unrounded) between the sums and the writes.  LayerNorm takes the mean first and then the squares of the
 // centred values, both from registers, so a row with a large mean loses nothing to cancellation.
-// 75,600 rows of 5120 in bf16 with modulation in fp32 (3.10 GB) take 500 us (6.2 TB/s, 0.94 of a copy).  A row takes
-// registers, so an SM holds 16 warps, and the row that each has on its way is what hides the latency (without it
-// 760 us).  CTAs of 128 threads, four on an SM: three 633, five 616 (spills), six 731; three of 256 threads 600.  The
+// 75,600 rows of 5120 in bf16 with modulation in fp32 (3.10 GB) take 500-551 us from box to box (5.6-6.2 TB/s, 0.86-0.94 of a
+// copy).  A row takes registers, so an SM holds 16 warps (12 where a warp holds a row of 1152), and the row that each has on
+// its way is what hides the latency (without it 760 us).  CTAs of 128 threads, four on an SM: three 633, five 616 (spills), six 731; three of 256 threads 600.  The
 // modulation's 60 KB a row come from L1, more bytes than the row's own 40 KB: 551 us while they came 16 bytes a load,
 // 610-637 with the row ahead in shared memory (five or six CTAs on an SM), which takes L1's room.
 #include <cstring>
@@ -275,7 +275,9 @@ __device__ __forceinline__ void normalise(const NormArgs& a, int how, E (&x)[VPT
 
 template <int TPR> constexpr int kRowsPerCta = TPR == 32 ? 4 : 1;
 
-// A row's vectors are requested while the row before it is worked on.
+// A row's vectors are requested while the row before it is worked on.  Four CTAs on an SM for five vectors in 128 threads are
+// the 16-bit types' best; fp32 rows of 4097-5120 values spill 192 bytes a thread there (75,600 of 5120 1576 us, 3.9 TB/s; of 4096
+// values, without a spill, 5.4).
 template <typename T, int V, int TPR, int VPT>
 __global__ void __launch_bounds__(TPR * kRowsPerCta<TPR>, TPR == 128 && VPT == 5 ? 4 : 1)
 gated_residual_norm_kernel(const __grid_constant__ NormArgs a) {

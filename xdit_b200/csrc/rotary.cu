@@ -13,7 +13,7 @@
 // the order in which they lie in memory (heads of a token, or tokens of a head, whichever are nearer), so that
 // loads and stores cover runs of 4 KB.  Tokens share a CTA because 64-bit angles cost more than a head's rotation does:
 // with every thread taking its own, q and k of 75,600 tokens x 40 heads of 128 in bf16 (3.10 GB) took 850 us; they take
-// 496 us (6.24 TB/s, 0.95 of a copy), half of the issue slots used.  Four vectors ahead of a thread in 128 registers were
+// 494-506 us (6.1-6.3 TB/s, 0.94-0.96 of a copy), half of the issue slots used.  Four vectors ahead of a thread in 128 registers were
 // slower than one ahead in 32 with seven CTAs on an SM.  A token or two are bound by the launch.
 #include <cstring>
 

@@ -57,10 +57,11 @@ def fp8_linear(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight, bias: Optiona
                quantize_out: bool = False) -> Union[torch.Tensor, Fp8Rows]:
     """``activation(x @ weight.T + bias)`` -> ``[..., N]``.
 
-    ``x``: a tensor ``[..., K]``, quantised by the rule of :func:`quantize_rows`, or :class:`Fp8Rows` with scales of any value.
-    ``activation``: ``None`` or ``"gelu_tanh"``.  ``out_dtype``: bf16, fp16 or fp32 (the dtype of ``x`` when it is a tensor, else
+    ``x``: a tensor ``[..., K]``, quantised by the rule of :func:`quantize_rows` (rows on 16-byte boundaries), or
+    :class:`Fp8Rows` with scales of any value.  ``activation``: ``None`` or ``"gelu_tanh"``.  ``out_dtype``: bf16, fp16 or fp32 (the dtype of ``x`` when it is a tensor, else
     bf16).  ``quantize_out``: the result as :class:`Fp8Rows` (N a multiple of 16), quantised from the fp32 sums.  The sums of
-    a block of 128 run in the tensor cores in fp32, their scaled sum in fp32 registers."""
+    a block of 128 run in the tensor cores in fp32, their scaled sum in fp32 registers; the product of two scales is taken in
+    fp32 too and has to be within its range."""
     w, ws = weight.data, weight.scale
     if isinstance(x, torch.Tensor):
         out_dtype = x.dtype if out_dtype is None else out_dtype

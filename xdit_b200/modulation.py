@@ -27,12 +27,13 @@ def gated_residual_norm(residual: torch.Tensor, branch: Optional[torch.Tensor] =
     returns ``(hidden, normed)``.
 
     ``residual`` and ``branch``: ``[B, s, C]`` in bf16, fp16 or fp32, contiguous last axis, C up to 16384.  Without a branch
-    ``hidden`` is ``residual`` itself.  ``norm`` and ``post_norm``: ``"layer"``, ``"rms"`` or ``None`` (``norm=None``: ``normed`` is
-    ``None``), each with an optional ``weight`` and ``bias`` ``[C]``.  ``gate``, ``scale`` and ``shift``: ``[C]``, ``[B, C]``, ``[B, 1, C]`` or,
+    ``hidden`` is ``residual`` itself, whatever ``residual_scale``.  ``norm`` and ``post_norm``: ``"layer"``, ``"rms"`` or ``None``
+    (``norm=None``: ``normed`` is ``None``), each with an optional ``weight`` and ``bias`` ``[C]``.  ``gate``, ``scale`` and ``shift``: ``[C]``, ``[B, C]``, ``[B, 1, C]`` or,
     for each token, ``[B, s, C]``.  Rows of parameters are in the tensors' dtype or fp32.  ``hidden`` is summed in fp32,
     rounded once where it is written, and ``norm`` takes the unrounded sum; ``out_residual`` (``residual`` or ``branch``
     itself, for an update in place; it must not overlap an input in another way) receives it.  With ``quantize`` ``normed`` is
-    an :class:`~xdit_b200.fp8_linear.Fp8Rows` for the 8-bit projection that follows (C a multiple of 16)."""
+    an :class:`~xdit_b200.fp8_linear.Fp8Rows` for the 8-bit projection that follows (C a multiple of 16, and all
+    rows, those of modulation too, on 16-byte boundaries)."""
     if residual.dim() != 3:
         raise ValueError("expected [B, s, C]")
     if torch.compiler.is_compiling() and out_residual is None:
