@@ -590,7 +590,8 @@ def _refuse_gradient(*tensors) -> None:
 
 def _check_tensors(first: torch.Tensor, *others) -> None:
     """What every launch asks of its tensors: no gradient to record, CUDA memory, one device."""
-    _refuse_gradient(first, *others)
+    if torch.is_grad_enabled() and (first.requires_grad or [t for t in others if t is not None and t.requires_grad]):
+        _refuse_gradient(first, *others)  # (looked at in line: a call of a few microseconds)
     if not first.is_cuda:
         _require_cuda(first)
     device = first.get_device()
