@@ -413,7 +413,8 @@ XDIT_API int xdit_gated_residual_norm(const struct xdit_norm_params* p, void* st
 /* e4m3 with one fp32 scale for each block of 128.  The scale is the smallest power of two that brings a
  * block within 448 (1 for a block of zeros, NaN for a block with an infinity or a NaN), so a value
  * is rounded once.  Rows: x [B, s, K] -> q [B*s, K], scale[block * scale_ld + row].  Weight: w [N, K] ->
- * q [N, K], scale [N/128 rounded up][K/128 rounded up], blocks of 128 x 128.  K % 16 == 0, 16-byte aligned rows. */
+ * q [N, K], scale [N/128 rounded up][K/128 rounded up], blocks of 128 x 128.  K % 16 == 0, 16-byte aligned rows; q
+ * and scale overlap nothing that is read. */
 XDIT_API int xdit_quantize_rows(const void* x, int64_t stride_b, int64_t stride_row, int32_t dtype, int32_t B,
                                 int32_t s, int32_t K, void* q, float* scale, int64_t scale_ld, void* stream);
 XDIT_API int xdit_quantize_weight(const void* w, int64_t stride_row, int32_t dtype, int32_t N, int32_t K, void* q,
@@ -422,7 +423,8 @@ XDIT_API int xdit_quantize_weight(const void* w, int64_t stride_row, int32_t dty
 /* out[m, n] = act(sum_c x_scale[m, c] w_scale[n/128, c] sum_{k in block c} x[m, k] w[n, k] + bias[n]) with x
  * [M, K] and w [N, K] in e4m3 and scales of any value whose products are within fp32's range.  out: bf16, fp16 or fp32, rounded once; or, with
  * out_q, e4m3 rows [M, N] with out_scale[block * out_scale_ld + row] (N % 16 == 0).  K % 16 == 0; rows of x and
- * w start on 16-byte boundaries.  status, status_host and wait_limit_ns as in xdit_attn_params.
+ * w start on 16-byte boundaries; the result overlaps no input but `raw`.  status, status_host and wait_limit_ns as
+ * in xdit_attn_params.
  * Replaces: the fp8 linear layers of xfuser/model_executor/layers/fp8_linear.py. */
 enum xdit_activation { XDIT_ACT_NONE = 0, XDIT_ACT_GELU_TANH = 1 };
 struct xdit_fp8_linear_params {

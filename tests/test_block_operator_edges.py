@@ -283,3 +283,43 @@ def test_norm_at_both_ends_of_every_width_of_vectors(C):
     zmag = (mag * r + wh.abs() * r * (mag * mag).mean(-1, keepdim=True) * r * r) * (1 + scale.double().abs())
     for got, want, m in ((h, wh, mag), (z, wz, zmag)):
         assert ((got.double() - want).abs() <= 128 * 2.0 ** -24 * m + want.abs() * 2.0 ** -8).all()
+
+
+# ---- e4m3 kernels: outputs in an input's place ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 200, 3000])
+def test_e4m3_kernels_refuse_results_in_an_input_s_place(M):
+    """Rows of x and of w are read for as long as any tile runs."""
+    from xdit_b200 import ops
+    from xdit_b200._capi import XditError
+    from xdit_b200.fp8_linear import quantize_rows, quantize_weight
+
+    g, K = torch.Generator(device="cuda").manual_seed(4), 1024
+    x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+    rows, w = quantize_rows(x), quantize_weight(torch.randn(K, K, device="cuda", generator=g))
+    q, s = ops.empty_fp8_rows(M, K, "cuda")
+    kept = [t.clone() for t in (rows.data.view(torch.uint8), rows.scale, w.data.view(torch.uint8), w.scale, x)]
+    for data, scale in ((rows.data, s), (q, rows.scale), (w.data[:M], s) if M <= K else (rows.data, s)):
+        with pytest.raises(XditError) as e:
+            ops.fp8_linear(rows.data, rows.scale, w.data, w.scale, out_q=data, out_scale=scale)
+        assert e.value.code == -2
+    lib, scale = _capi.load(), s.data_ptr()
+    assert lib.xdit_quantize_rows(x.data_ptr(), 0, K, 0, 1, M, K, x.data_ptr(), scale, M, None) == -2
+    assert lib.xdit_quantize_weight(x.data_ptr(), K, 0, M, K, x.data_ptr(), scale, None) == -2
+    torch.cuda.synchronize()
+    for a, b in zip(kept, (rows.data.view(torch.uint8), rows.scale, w.data.view(torch.uint8), w.scale, x)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_result_in_the_place_of_an_input_that_the_call_quantises():
+    from xdit_b200 import ops
+    from xdit_b200.fp8_linear import fp8_linear, quantize_weight
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = quantize_weight(torch.randn(1024, 1024, device="cuda", generator=g) / 32)
+    for M in (3, 300, 9000):
+        x = torch.randn(M, 1024, device="cuda", generator=g).bfloat16()
+        want = fp8_linear(x, w)
+        ops.fp8_linear(x.unsqueeze(0), None, w.data, w.scale, out=x)
+        assert torch.equal(x, want)

@@ -967,6 +967,11 @@ extern "C" int xdit_fp8_linear(const struct xdit_fp8_linear_params* p, void* str
       return XDIT_E_KERNEL_TIMEOUT;
     }
   }
+  const void* result = p->out_q ? p->out_q : p->out;
+  if (result == p->x || result == p->w || (p->out_q && (p->out_scale == p->x_scale || p->out_scale == p->w_scale))) {
+    set_error("%s: the result lies on x, w or their scales, which are read until the last tile is done", who);
+    return XDIT_E_SHAPE;
+  }
   int sms = 0;
   int rc = check_device(&sms);
   if (rc) return rc;

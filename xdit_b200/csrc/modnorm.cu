@@ -678,6 +678,7 @@ int launch_quantize_rows(const char* who, const void* x, int64_t stride_b, int64
     set_error("%s: rows must start on 16-byte boundaries", who);
     return XDIT_E_ALIGN;
   }
+  if (x == q) { set_error("%s: the e4m3 rows lie on those that are read", who); return XDIT_E_SHAPE; }
   int rc = check_device(nullptr);
   if (rc) return rc;
   const int grid = (int)(rows < 0x7fffffffll ? rows : 0x7fffffffll);
@@ -723,6 +724,7 @@ int xdit_quantize_weight(const void* w, int64_t stride_row, int32_t dtype, int32
   }
   const int64_t blocks = (int64_t)((N + kBlock - 1) / kBlock) * ((K + kBlock - 1) / kBlock);
   if (blocks > 0x7fffffffll) { set_error("%s: too many blocks", who); return XDIT_E_SHAPE; }
+  if (w == q) { set_error("%s: the e4m3 weight lies on the one that is read", who); return XDIT_E_SHAPE; }
   int rc = check_device(nullptr);
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
