@@ -63,7 +63,7 @@ def _seq(t: Optional[torch.Tensor]) -> _capi.Seq:
 
 
 class _Status:
-    """Per-device pair of status words of the attention kernel: ``dev`` (int32 in device memory, read
+    """Per-device pair of status words of the kernels with bounded waits (attention, 8-bit linear layers): ``dev`` (int32 in device memory, read
     by every launch) and ``host`` (int32 in pinned, device-mapped host memory, written by a launch
     only when one of its bounded waits gave up, and read by the C entry point before it launches)."""
 
@@ -87,7 +87,7 @@ def _status(device) -> _Status:
 
 
 def status_buffer(device) -> torch.Tensor:
-    """Per-device int32 word the attention kernel sets when one of its bounded waits gives up."""
+    """Per-device int32 word that a kernel sets when one of its bounded waits gives up."""
     return _status(device).dev
 
 
@@ -99,12 +99,12 @@ def clear_status(device=None) -> None:
 
 
 def check_status(device=None) -> None:
-    """Synchronise and raise if any attention kernel on ``device`` (the current device for a bare
+    """Synchronise and raise if any kernel with bounded waits on ``device`` (the current device for a bare
     ``"cuda"``; every device used so far when None) reported a timed-out wait.  The words are cleared
     before the exception is raised, so that later launches run again.
 
     Product calls do not need this: a failure also lands in a host-visible word that the next
-    ``xdit_attn_fwd`` call reads without synchronising, and that call raises
+    ``xdit_attn_fwd`` or ``xdit_fp8_linear`` call reads without synchronising, and that call raises
     ``XditError(XDIT_E_KERNEL_TIMEOUT)`` (see :func:`attn_fwd`).  This function is for the end of a
     run, where no next call follows."""
     sts = list(_status_bufs.values()) if device is None else [_status_bufs.get(_device_index(device))]
