@@ -63,8 +63,8 @@ def _seq(t: Optional[torch.Tensor]) -> _capi.Seq:
 
 
 class _Status:
-    """Per-device pair of status words of the kernels with bounded waits (attention, 8-bit linear layers): ``dev`` (int32 in device memory, read
-    by every launch) and ``host`` (int32 in pinned, device-mapped host memory, written by a launch
+    """Per-device pair of status words of the kernels with bounded waits (attention, 8-bit linear layers): ``dev`` (int32 in
+    device memory, read by every launch) and ``host`` (int32 in pinned, device-mapped host memory, written by a launch
     only when one of its bounded waits gave up, and read by the C entry point before it launches)."""
 
     def __init__(self, index: int):
